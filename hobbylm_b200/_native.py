@@ -28,6 +28,8 @@ EXPORTS = (
     "hg_decode_greedy", "hg_engine_stream", "hg_decode_kernel_count", "hg_debug_time_attention",
     "hg_op_q8_matvec_noalloc", "hg_host_sample", "hg_host_score_block", "hg_generate_embeds",
     "hg_ep_unique_id", "hg_engine_ep_init",
+    "hg_kv8_block_bytes", "hg_op_kv8_append", "hg_op_kv8_read", "hg_op_kv8_attn_scratch_bytes", "hg_op_kv8_attn",
+    "hg_op_logits_rules",
 )
 NOALLOC_SCRATCH_BYTES = 4 << 20  # HG_NOALLOC_SCRATCH_BYTES
 
@@ -79,6 +81,33 @@ class KvAttnArgs(C.Structure):
                                                          "block_table")] + [
         ("bt_stride", C.c_int32), ("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("page_stride", C.c_int64),
         ("out", C.c_void_p)]
+
+
+class Kv8Cache(C.Structure):
+    """hg_kv8_cache: one layer's 8-bit paged KV pool."""
+    _fields_ = [(n, C.c_int32) for n in ("n_kv_heads", "head_dim", "n_pages", "bt_stride")] + [
+        ("block_table", C.c_void_p), ("pool", C.c_void_p), ("page_stride", C.c_int64)]
+
+
+class Rows(C.Structure):
+    """hg_rows: the rows of a ragged batch, chains or drafted trees."""
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "n_rows", "max_rows")] + [
+        (n, C.c_void_p) for n in ("row_off", "start", "parent", "err")]
+
+
+class Kv8Append(C.Structure):
+    """hg_kv8_append_args."""
+    _fields_ = [("n_heads", C.c_int32), ("max_pos", C.c_int32), ("eps", C.c_float)] + [
+        (n, C.c_void_p) for n in ("qkv", "q_norm", "k_norm", "rope_cos", "rope_sin", "q_out")]
+
+
+class LogitsRules(C.Structure):
+    """hg_logits_rules_args."""
+    _fields_ = [("vocab", C.c_int32), ("valid", C.c_int32), ("logits", C.c_void_p), ("out", C.c_void_p),
+                ("ld", C.c_int64), ("ld_out", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("next_ids", "token", "hist_off", "hist", "rep_penalty", "freq_penalty",
+                                  "pres_penalty", "bias_off", "bias_id", "bias", "mask", "mask_row")] + [
+        ("mask_words", C.c_int32)]
 
 
 TOKEN_CB = C.CFUNCTYPE(C.c_int, C.c_uint32, C.c_void_p)
@@ -138,6 +167,12 @@ def lib():
         "hg_ep_unique_id": (i32, [vp]),
         "hg_engine_ep_init": (i32, [vp, vp, i32, i32]),
         "hg_decode_kernel_count": (i32, [vp, i32]),
+        "hg_kv8_block_bytes": (i64, [i32]),
+        "hg_op_kv8_append": (i32, [C.POINTER(Kv8Cache), C.POINTER(Rows), C.POINTER(Kv8Append), vp]),
+        "hg_op_kv8_read": (i32, [C.POINTER(Kv8Cache), C.POINTER(Rows), vp, vp, vp]),
+        "hg_op_kv8_attn_scratch_bytes": (sz, [C.POINTER(Kv8Cache), C.POINTER(Rows), i32]),
+        "hg_op_kv8_attn": (i32, [C.POINTER(Kv8Cache), C.POINTER(Rows), i32, vp, vp, vp, vp]),
+        "hg_op_logits_rules": (i32, [C.POINTER(Rows), C.POINTER(LogitsRules), vp]),
         "hg_debug_time_attention": (i32, [vp, vp, i32, i32, C.POINTER(f32), C.POINTER(f32)]),
     }
     for name, (res, args) in sig.items():

@@ -19,8 +19,9 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libhobbygpu.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
-SOURCES = ["engine.cu", "decode.cu", "tc.cu", "ep.cu", "prefill.cu", "sample.cu", "noalloc.cu", "gguf.cpp", "sampler.cpp"]
-HEADERS = ["hg_device.cuh", "hg_model.cuh", "hg_launch.h", "hg_host.h", "hg_ep.h"]
+SOURCES = ["engine.cu", "decode.cu", "tc.cu", "ep.cu", "prefill.cu", "sample.cu", "noalloc.cu", "kv8.cu", "kv8_attn.cu",
+           "rules.cu", "gguf.cpp", "sampler.cpp"]
+HEADERS = ["hg_device.cuh", "hg_model.cuh", "hg_launch.h", "hg_host.h", "hg_ep.h", "hg_kv8.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # --fmad=false: no implicit FMA contraction; kernels write every fused multiply-add explicitly so the

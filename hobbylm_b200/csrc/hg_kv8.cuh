@@ -1,0 +1,142 @@
+// Shared pieces of the 8-bit KV cache kernels (kv8.cu, kv8_attn.cu) and the logit rules (rules.cu):
+// the argument structs as the kernels see them, the checks of row and page indices that come from
+// device memory, and the host-side argument checks of the entry points.
+#pragma once
+#include <climits>
+#include <string>
+
+#include "hg_device.cuh"
+#include "hg_host.h"
+
+namespace hg {
+
+constexpr int KV8_PAGE = 16;           // slots of a page
+constexpr int KV8_MAX_SEQS = 1024;     // sequences of one call
+constexpr int KV8_MAX_GROUP = 32;      // q heads per kv head
+
+__host__ __device__ constexpr int kv8_block_bytes(int hd) { return 32 * hd + 128; }
+
+// Byte offsets inside a (page, kv head) block (hobbygpu.h, hg_kv8_cache). The K tile of 8 slots x 16
+// bytes and the V column of 16 slots are the 128-byte core matrices that a tcgen05 operand without
+// swizzle is made of, so a page goes into shared memory by plain bulk copies, ready for the MMA.
+__host__ __device__ constexpr int kv8_k_off(int hd, int w, int i) {
+  return (w >> 3) * 8 * hd + (i >> 4) * 128 + (w & 7) * 16 + (i & 15);
+}
+__host__ __device__ constexpr int kv8_v_off(int hd, int w, int i) { return 16 * hd + i * 16 + w; }
+__host__ __device__ constexpr int kv8_ks_off(int hd, int w) { return 32 * hd + 4 * w; }
+__host__ __device__ constexpr int kv8_vs_off(int hd, int w) { return 32 * hd + 64 + 4 * w; }
+
+__device__ __forceinline__ void kv8_flag(int32_t* err, int code) {
+  if (err) atomicExch(err, code);
+}
+
+// The rows of a sequence, with the offsets clamped to the row buffers: [r0, r0 + n), behind `start`.
+struct SeqSpan {
+  int r0, n, start;
+};
+__device__ __forceinline__ SeqSpan kv8_span(const hg_rows& R, int s, bool with_start) {
+  SeqSpan p;
+  const int a = R.row_off[s], b = R.row_off[s + 1];
+  p.r0 = min(max(a, 0), R.n_rows);
+  p.n = min(max(b, p.r0), R.n_rows) - p.r0;
+  p.start = with_start ? R.start[s] : 0;
+  if (p.start < 0 || p.n > R.max_rows || a < 0 || b < a || b > R.n_rows) {
+    kv8_flag(R.err, HG_ERR_INVALID);
+    p.n = p.start < 0 ? 0 : min(p.n, R.max_rows);
+  }
+  return p;
+}
+
+// The parent of row j of a span (-1: none, -2: row j is padding); one that is not below j is none.
+__device__ __forceinline__ int kv8_parent(const hg_rows& R, const SeqSpan& p, int j) {
+  if (!R.parent) return j - 1;
+  const int q = R.parent[p.r0 + j];
+  if (q < j) return max(q, -2);
+  kv8_flag(R.err, HG_ERR_INVALID);
+  return -1;
+}
+
+// Address of the block of (slot, kv head), or null where the sequence has no such page. Slots are
+// 64-bit: start + j may pass the 32-bit range.
+__device__ __forceinline__ uint8_t* kv8_block(const hg_kv8_cache& C, int s, long long slot, int kvh) {
+  const long long pg = slot / KV8_PAGE;
+  if (pg >= C.bt_stride) return nullptr;
+  const int id = C.block_table[(size_t)s * C.bt_stride + pg];
+  if ((unsigned)id >= (unsigned)C.n_pages) return nullptr;
+  return static_cast<uint8_t*>(C.pool) + (long long)id * C.page_stride + (long long)kvh * kv8_block_bytes(C.head_dim);
+}
+
+// ---- host ----
+inline void kv8_need(bool ok, const char* what) {
+  if (!ok) throw Error(HG_ERR_INVALID, what);
+}
+inline bool kv8_aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+inline void kv8_check_rows(const hg_rows* r, bool with_start) {
+  kv8_need(r, "null argument");
+  kv8_need(r->n_seqs >= 0 && r->n_seqs <= KV8_MAX_SEQS, "n_seqs must be in 0..1024");
+  kv8_need(r->n_rows >= 0 && r->n_rows <= INT_MAX / 256, "n_rows out of range");
+  if (r->n_seqs == 0 || r->n_rows == 0) return;
+  kv8_need(r->max_rows > 0, "max_rows must be positive");
+  kv8_need(r->row_off && (r->start || !with_start), "null argument");
+  kv8_need(kv8_aligned(r->row_off, 4) && kv8_aligned(r->start, 4) && kv8_aligned(r->parent, 4) &&
+               kv8_aligned(r->err, 4),
+           "row arrays must be 4-byte aligned");
+}
+
+inline void kv8_check_cache(const hg_kv8_cache* c) {
+  kv8_need(c, "null argument");
+  kv8_need(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
+  kv8_need(c->n_kv_heads > 0 && c->n_kv_heads <= 1024, "n_kv_heads must be in 1..1024");
+  kv8_need(c->n_pages > 0, "n_pages must be positive");
+  kv8_need(c->bt_stride > 0 && c->bt_stride <= INT_MAX / KV8_PAGE, "bt_stride out of range");
+  kv8_need(c->block_table && c->pool, "null argument");
+  kv8_need(kv8_aligned(c->block_table, 4), "block_table must be 4-byte aligned");
+  kv8_need(kv8_aligned(c->pool, 16), "pool must be 16-byte aligned");
+  kv8_need(c->page_stride % 16 == 0 && c->page_stride >= (int64_t)c->n_kv_heads * kv8_block_bytes(c->head_dim),
+           "page_stride must be a multiple of 16 and hold a page's blocks");
+}
+
+// The device that holds p becomes current for the call.
+struct Kv8Device {
+  int prev = -1;
+  explicit Kv8Device(const void* p) {
+    cudaPointerAttributes at{};
+    cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      throw Error(HG_ERR_CUDA, std::string("cudaPointerGetAttributes: ") + cudaGetErrorString(e));
+    }
+    kv8_need(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "not device memory");
+    int cur = -1;
+    cudaGetDevice(&cur);
+    if (cur != at.device) {
+      e = cudaSetDevice(at.device);
+      if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+      prev = cur;
+    }
+  }
+  ~Kv8Device() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  Kv8Device(const Kv8Device&) = delete;
+  Kv8Device& operator=(const Kv8Device&) = delete;
+};
+
+inline void kv8_launched(cudaError_t e) {
+  if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
+}
+
+#define KV8_API(...)                                     \
+  try {                                                  \
+    __VA_ARGS__;                                         \
+    return HG_OK;                                        \
+  } catch (const ::hg::Error& ex_) {                     \
+    ::hg::set_last_error(ex_.what());                    \
+    return ex_.code;                                     \
+  } catch (const std::exception& ex_) {                  \
+    ::hg::set_last_error(ex_.what());                    \
+    return HG_ERR_INVALID;                               \
+  }
+
+}  // namespace hg

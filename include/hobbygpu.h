@@ -318,6 +318,114 @@ typedef struct {
 size_t hg_op_kv_attn_scratch_bytes(const hg_kv_attn_args* a);
 int hg_op_kv_attn(const hg_kv_attn_args* a, void* scratch, void* stream);
 
+/* ---- 8-bit KV cache, drafted token trees and logit rules (device pointers) ----
+ *
+ * No counterpart in the reference (hobby-rs keeps f32 K/V, decodes one token at a time and samples on
+ * the host). One step of speculative decoding over these entry points: hg_op_kv8_append writes the
+ * drafted rows of every sequence behind its context, hg_op_kv8_attn attends them (each row sees the
+ * context, itself and its ancestors in the draft), hg_op_logits_rules turns the rows' logits into
+ * constrained ones with a greedy pick each; the accepted rows are then appended again as a chain.
+ * One row per sequence is ordinary batched decode.
+ *
+ * Pointers in these structs are device memory, 4-byte aligned (float rows read or written whole 16-byte
+ * aligned); the call runs on the device that holds the pool (for the rules: the logits). Arrays in
+ * device memory are checked on the device: what breaks a rule is left out as described, and *err, when
+ * given, is set to an HG_ERR_* code and never cleared. Calls neither allocate nor synchronise, and can
+ * be captured into a CUDA graph. */
+
+/* The cache of one layer. Pages hold 16 slots; the block of kv head h in page p starts at
+ * pool + p * page_stride + h * hg_kv8_block_bytes(head_dim) and holds, for slot w = 0..15 and dim i:
+ *   K codes, int8, at (w / 8) * 8 * head_dim + (i / 16) * 128 + (w % 8) * 16 + i % 16
+ *   V codes, int8, at 16 * head_dim + i * 16 + w
+ *   K scales, f32 [16], at 32 * head_dim, and V scales, f32 [16], at 32 * head_dim + 64
+ * A value is code * scale, |code| <= 127; a row with a NaN or an infinity has scale NaN. */
+typedef struct {
+  int32_t n_kv_heads, head_dim;  /* head_dim 64 or 128 */
+  int32_t n_pages;               /* pages of the pool: a table entry outside 0..n_pages-1 is no page */
+  int32_t bt_stride;             /* table entries per sequence */
+  const int32_t* block_table;    /* [n_seqs][bt_stride] page ids */
+  void* pool;                    /* 16-byte aligned */
+  int64_t page_stride;           /* bytes, a multiple of 16, at least n_kv_heads blocks */
+} hg_kv8_cache;
+
+/* Rows of a ragged batch: rows row_off[s]..row_off[s+1]-1 belong to sequence s, and its row j goes to
+ * slot start[s] + j, behind the slots it holds already. parent[row] is the index j' < j (within the
+ * sequence) of the row drafted before it, -1 for a row that follows the context, -2 for a padding row
+ * (in no tree: not cached, seen by no row, a child of it sees only itself and the context). parent =
+ * NULL: every row follows the one before it. The position of a row is start[s] plus its number of
+ * ancestors. Rows from row_off[n_seqs] on are left as they were. A parent that is not below its row
+ * counts as -1 (err HG_ERR_INVALID); rows past max_rows of a sequence, and sequences with start < 0,
+ * are left out (err HG_ERR_INVALID). */
+typedef struct {
+  int32_t n_seqs, n_rows;   /* sequences (at most 1024); rows of the row-wise buffers */
+  int32_t max_rows;         /* no sequence has more rows than this */
+  const int32_t* row_off;   /* [n_seqs + 1] */
+  const int32_t* start;     /* [n_seqs] (hg_op_logits_rules: unused) */
+  const int32_t* parent;    /* [n_rows] or NULL */
+  int32_t* err;             /* one word, or NULL */
+} hg_rows;
+
+/* Bytes of one kv head's block of a page: 32 * head_dim + 128 (0 for another head_dim). */
+int64_t hg_kv8_block_bytes(int head_dim);
+
+/* QK-norm + RoPE of every row's q and k heads (model.rs:199-208), and its k and v heads quantized into
+ * the cache: per row and head scale = max|x| / 127 in f32 and code = round-half-even(x / scale), k
+ * computed in f64 so that no code depends on a summation order. A row without a page or with a position
+ * >= max_pos is not cached and its q_out row is zeros (err HG_ERR_CONTEXT); padding rows' q_out: zeros. */
+typedef struct {
+  int32_t n_heads, max_pos;
+  float eps;
+  const float* qkv;        /* [n_rows][(n_heads + 2 n_kv_heads) * head_dim] pre-norm projections */
+  const float* q_norm;     /* [head_dim] */
+  const float* k_norm;     /* [head_dim] */
+  const float* rope_cos;   /* [max_pos][head_dim / 2] (hg_rope_tables) */
+  const float* rope_sin;
+  float* q_out;            /* [n_rows][n_heads * head_dim], or NULL */
+} hg_kv8_append_args;
+int hg_op_kv8_append(const hg_kv8_cache* c, const hg_rows* r, const hg_kv8_append_args* a, void* stream);
+
+/* The cached K and V (either may be NULL) of the rows' slots as f32 [n_rows][n_kv_heads * head_dim];
+ * zeros where there is no page (err HG_ERR_CONTEXT). parent is not used. */
+int hg_op_kv8_read(const hg_kv8_cache* c, const hg_rows* r, float* k_out, float* v_out, void* stream);
+
+/* Attention of every row's q heads (normed and roped, as hg_op_kv8_append writes them) over the slots it
+ * sees: 0..start[s]-1, its ancestors' and its own (the rows are in the cache already), softmax of
+ * q . k / sqrt(head_dim). q, out: [n_rows][n_heads * head_dim] f32, n_heads / n_kv_heads at most 32.
+ * Slots without a page are not seen (err HG_ERR_CONTEXT); a row that sees nothing gets zeros. scratch:
+ * 16-byte aligned device buffer of hg_op_kv8_attn_scratch_bytes() bytes, its content of no meaning
+ * before and after the call; calls that may overlap need one each. */
+size_t hg_op_kv8_attn_scratch_bytes(const hg_kv8_cache* c, const hg_rows* r, int n_heads);
+int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_heads, const float* q, float* out, void* scratch,
+                   void* stream);
+
+/* Rules on the rows' logits, in this order: the repetition penalty once per occurrence of an id among
+ * the sequence's history and the drafted tokens on the row's path (l > 0: l / p, else l * p, as
+ * lib.rs:130-139); minus freq_penalty * occurrences; minus pres_penalty if it occurs; plus the sequence's
+ * bias (an id listed more than once: the sum, added up in the list's order); -inf for ids >= valid and for ids whose
+ * bit of the row's mask is 0. next_ids: the first greatest logit (NaN never wins), -1 if none is above
+ * -inf. Ids outside 0..vocab-1 in the lists are passed over. A padding row's logits are left as they
+ * were, its next id is -1. out may be logits itself (same row stride). */
+typedef struct {
+  int32_t vocab, valid;          /* valid <= 0: every id */
+  const float* logits;           /* [n_rows] rows of vocab floats */
+  float* out;
+  int64_t ld, ld_out;            /* floats between rows (0: vocab) */
+  int32_t* next_ids;             /* [n_rows] or NULL */
+  const int32_t* token;          /* [n_rows] the drafted token of each row, or NULL (none counted) */
+  const int32_t* hist_off;       /* [n_seqs + 1] or NULL */
+  const int32_t* hist;           /* ids */
+  const float* rep_penalty;      /* [n_seqs] each, or NULL */
+  const float* freq_penalty;
+  const float* pres_penalty;
+  const int32_t* bias_off;       /* [n_seqs + 1] or NULL */
+  const int32_t* bias_id;
+  const float* bias;
+  const uint32_t* mask;          /* rows of mask_words words, bit i % 32 of word i / 32 = id i is allowed; or NULL */
+  const int32_t* mask_row;       /* [n_rows] mask row of each row, negative: none; NULL: row i has mask row i */
+  int32_t mask_words;            /* at least vocab / 32, rounded up */
+} hg_logits_rules_args;
+int hg_op_logits_rules(const hg_rows* r, const hg_logits_rules_args* a, void* stream);
+
 /* Rope::new tables (ops.rs:139-154), computed on the host in f64: cos/sin [max_pos][head_dim/2]. */
 int hg_rope_tables(int head_dim, int max_pos, float theta, float* cos_out, float* sin_out);
 

@@ -21,7 +21,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["engine.cu", "decode.cu", "tc.cu", "ep.cu", "prefill.cu", "sample.cu", "noalloc.cu", "kv8.cu", "kv8_attn.cu",
            "rules.cu", "gguf.cpp", "sampler.cpp"]
-HEADERS = ["hg_device.cuh", "hg_model.cuh", "hg_launch.h", "hg_host.h", "hg_ep.h", "hg_kv8.cuh"]
+HEADERS = ["hg_device.cuh", "hg_model.cuh", "hg_launch.h", "hg_host.h", "hg_ep.h", "hg_kv8.cuh", "hg_tc.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # --fmad=false: no implicit FMA contraction; kernels write every fused multiply-add explicitly so the

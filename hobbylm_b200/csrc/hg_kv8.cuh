@@ -89,7 +89,7 @@ inline void kv8_check_cache(const hg_kv8_cache* c) {
   kv8_need(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
   kv8_need(c->n_kv_heads > 0 && c->n_kv_heads <= 1024, "n_kv_heads must be in 1..1024");
   kv8_need(c->n_pages > 0, "n_pages must be positive");
-  kv8_need(c->bt_stride > 0 && c->bt_stride <= INT_MAX / KV8_PAGE, "bt_stride out of range");
+  kv8_need(c->bt_stride > 0 && c->bt_stride <= 1 << 26, "bt_stride out of range");
   kv8_need(c->block_table && c->pool, "null argument");
   kv8_need(kv8_aligned(c->block_table, 4), "block_table must be 4-byte aligned");
   kv8_need(kv8_aligned(c->pool, 16), "pool must be 16-byte aligned");
@@ -99,7 +99,7 @@ inline void kv8_check_cache(const hg_kv8_cache* c) {
 
 // The device that holds p becomes current for the call.
 struct Kv8Device {
-  int prev = -1;
+  int prev = -1, device = 0;
   explicit Kv8Device(const void* p) {
     cudaPointerAttributes at{};
     cudaError_t e = cudaPointerGetAttributes(&at, p);
@@ -108,6 +108,7 @@ struct Kv8Device {
       throw Error(HG_ERR_CUDA, std::string("cudaPointerGetAttributes: ") + cudaGetErrorString(e));
     }
     kv8_need(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "not device memory");
+    device = at.device;
     int cur = -1;
     cudaGetDevice(&cur);
     if (cur != at.device) {

@@ -33,10 +33,9 @@ namespace hg {
 
 constexpr int KA_TILE = 128;                      // slots of a tile: the MMA's M
 constexpr int KA_PAGES = KA_TILE / KV8_PAGE;      // pages of a tile
-constexpr int KA_COMPUTE = 128;                   // threads that hold a slot (S) or a dim (O)
-constexpr int KA_THREADS = KA_COMPUTE + 32;       // and the copy warp
 constexpr int KA_SMS = 148;
 constexpr int KA_MAX_CTAS = 3 * KA_SMS;
+constexpr float KA_NONE = -1e30f;                 // maximum of a row that has seen nothing: finite, below any score
 constexpr float KA_FIX = 8323072.0f;              // 2^23 - 2^16: the greatest fixed-point value, three digits
 
 // Shared memory of one CTA, in order: the ring, the digits of q and of the probabilities, small arrays.
@@ -44,24 +43,33 @@ template <int HD, int R>
 struct KaShape {
   static constexpr int N = (3 * R + 15) / 16 * 16;  // MMA N: digit columns
   static constexpr int NB = (3 * R + 7) / 8 * 8;    // digit rows kept (what N reads past them stays unread)
+  // bytes between 16-byte columns of the digit operands: 16 more than the rows take, so that the two
+  // columns that a warp's 32 slots lie in use different banks
+  static constexpr int PITCH = NB * 16 + 16;
   static constexpr int KBYTES = KA_TILE * HD, STAGE = 2 * KBYTES + KA_PAGES * 128;
   static constexpr int STAGES = HD == 128 ? 2 : 4;
-  static constexpr int OFF_BQ = STAGES * STAGE, OFF_BP = OFF_BQ + NB * HD, OFF_SMALL = OFF_BP + NB * KA_TILE;
+  static constexpr int OFF_BQ = STAGES * STAGE, OFF_BP = OFF_BQ + PITCH * (HD / 16),
+                       OFF_SMALL = OFF_BP + PITCH * (KA_TILE / 16);
   // tensor-memory columns: S at 0, O behind it; a power of two of at least 32
   static constexpr int COL_O = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;
   static constexpr int COLS = 2 * COL_O;
-  static constexpr int RC = R < 16 ? R : 16;  // rows per tensor-memory read
+  // Compute warps: groups of 128 threads, one slot (S) or dim (O) per thread and RT rows per group; and
+  // the copy warp.
+  static constexpr int GROUPS = R > 16 ? R / 16 : 1, RT = R / GROUPS, COMPUTE = 128 * GROUPS, THREADS = COMPUTE + 32;
+  static constexpr int RC = RT < 8 ? RT : 8;  // rows per tensor-memory read
+  static constexpr int PER_SM = R > 16 ? 2 : 3;
 };
 
 template <int R>
 struct KaSmall {
   uint64_t full[4], empty[4], sbar, obar;
-  float wmax[R][4];          // per warp maxima of a tile's scores
-  float wsum[R][4];          // per warp sums at a unit's end
-  float qs[R];               // row r: log2(e) / sqrt(hd) * q scale
-  int lim[R];                // row r sees the slots below, and the tree slots of `vis`
+  float wmax[4][R];          // per warp maxima of a tile's scores
+  float wsum[4][R];          // per warp sums at a unit's end
+  float qs[R];               // row r: 256 log2(e) / sqrt(hd) * q scale
+  int lim[R];                // row r sees the slots below, and the tree slots of `vis`; -1: padding
+  int node[R], off[R];       // row r's node within its block, its q head's place behind the block's first
   uint32_t vis[R][4];        // slots of the current tile that row r's path holds
-  float wsv[4];
+  float wsv[R > 16 ? R / 16 : 1][4];
   uint32_t pages[4];         // per stage: which of the tile's pages are there
   uint32_t tmem;
   int fail;
@@ -87,7 +95,8 @@ __device__ __forceinline__ float warp_fmax(float v) {  // NaN only if every lane
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bar_named(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(dst)),
@@ -97,22 +106,52 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ void mbar_arrive_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-// The three base-256 digits of a rounded sum, exact in f32 each, put together with one rounding each.
-__device__ __forceinline__ float digits(uint32_t d0, uint32_t d1, uint32_t d2) {
-  return __fmaf_rn(tc_isum(d2), 65536.0f, __fmaf_rn(tc_isum(d1), 256.0f, tc_isum(d0)));
+// A sum whose base-256 digits are d0, d1, d2 (each below 2^21.01 in magnitude). The upper two are put
+// together as integers and converted with one rounding. ka_score drops the lowest 8 of some 30 bits and
+// returns the sum / 256; ka_add adds the sum * f to acc with d0 in full (a dropped part would add up
+// over the tiles).
+__device__ __forceinline__ float ka_score(uint32_t d0, uint32_t d1, uint32_t d2) {
+  return __int2float_rn((int)((d2 << 8) + d1) + ((int)d0 >> 8));
+}
+__device__ __forceinline__ float ka_add(uint32_t d0, uint32_t d1, uint32_t d2, float f, float f256, float acc) {
+  return __fmaf_rn(__int2float_rn((int)((d2 << 8) + d1)), f256, __fmaf_rn(tc_isum(d0), f, acc));
+}
+// Sums over the warp of R values per lane: lane i < R gets value i's.
+template <int R>
+__device__ __forceinline__ float warp_sums(float (&v)[R]) {
+  const int lane = threadIdx.x & 31;
+  int o = R / 2;
+#pragma unroll
+  for (int half = R / 2; half > 0; half /= 2, o /= 2) {
+#pragma unroll
+    for (int i = 0; i < half; i++) {
+      const bool up = lane & o;
+      const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (int x = R; x < 32; x *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], x);
+  return v[0];
 }
 // Fixed point v (|v| <= KA_FIX) as signed digits v = b0 + 256 b1 + 65536 b2, one per byte.
 __device__ __forceinline__ uint32_t to_digits(uint32_t v) { return (v + 0x808080u) ^ 0x808080u; }
 
+// 8 consecutive tensor-memory columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+// The three digit columns of RC rows: digit i of row r is column i * stride + r.
 template <int RC>
 __device__ __forceinline__ void tmem_rows(uint32_t t, uint32_t stride, uint32_t (&d)[3][RC]) {
-  if constexpr (RC == 16) {
+  if constexpr (RC == 8) {
 #pragma unroll
-    for (int i = 0; i < 3; i++) tmem_ld16(t + i * stride, d[i]);
+    for (int i = 0; i < 3; i++) tmem_ld8(t + i * stride, d[i]);
   } else {
-    uint32_t v[32];
+    uint32_t v[16];  // the stride is RC: one read has them all
     tmem_ld16(t, v);
-    if (RC == 8) tmem_ld16(t + 16, v + 16);
 #pragma unroll
     for (int i = 0; i < 3 * RC; i++) d[i / RC][i % RC] = v[i];
   }
@@ -165,9 +204,9 @@ __device__ __forceinline__ bool ka_wait(uint64_t* bar, uint32_t parity, int* fai
 }
 
 template <int HD, int R>
-__global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const __grid_constant__ KaArgs A) {
+__global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_SM) k_kv8_attn(const __grid_constant__ KaArgs A) {
   using S = KaShape<HD, R>;
-  constexpr int STAGES = S::STAGES, E = HD / 32;
+  constexpr int STAGES = S::STAGES, E = HD / 32, RT = S::RT, COPY = S::COMPUTE / 32;
   extern __shared__ __align__(128) unsigned char ka_raw[];
   unsigned char* bq = ka_raw + S::OFF_BQ;
   unsigned char* bp = ka_raw + S::OFF_BP;
@@ -178,10 +217,14 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
   pdl_trigger();
 
   // ---- the line of tiles: first tile of each sequence ----
-  for (int s = tid; s < n_seqs; s += KA_THREADS) {
+  for (int s = tid; s < n_seqs; s += S::THREADS) {
     const SeqSpan sp = kv8_span(A.R, s, true);
     if ((long long)sp.start + sp.n > ka_cap(A.C)) kv8_flag(A.R.err, HG_ERR_CONTEXT);
     pre[s + 1] = (uint32_t)ka_tiles(A.C, sp) * A.C.n_kv_heads * ((sp.n + A.npb - 1) / A.npb);
+  }
+  if (tid < R) {
+    sm.node[tid] = tid / A.g;
+    sm.off[tid] = sm.node[tid] * A.nh + tid % A.g;
   }
   if (tid == 0) {
     pre[0] = 0;
@@ -216,7 +259,7 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
   if (cta >= G) return;
   const int begin = (int)(T * cta / G), end = (int)(T * (cta + 1) / G);
 
-  if (warp == KA_COMPUTE / 32) {
+  if (warp == COPY) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
                  "r"(S::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -226,7 +269,7 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
   tc_fence_after();
   const uint32_t tm = sm.tmem;
 
-  if (warp == KA_COMPUTE / 32) {
+  if (warp == COPY) {
     // =================== copy warp: lanes 0..7 fetch a page of the tile each ===================
     int n = 0;
     for (int t = begin; t < end;) {
@@ -264,8 +307,15 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
     for (int i = max(0, n - STAGES); i < n; i++) mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1);
   } else {
     // =================== compute warps ===================
-    const uint32_t tq = tm + ((uint32_t)(warp * 32) << 16);
-    unsigned char* bp_mine = bp + (tid >> 4) * (S::NB * 16) + (tid & 15);
+    // this thread: slot / dim ti of the tile, rows rb .. rb + RT - 1
+    const int ti = tid & 127, quad = warp & 3, grp = warp >> 2, rb = grp * RT;
+    const uint32_t tq = tm + ((uint32_t)(quad * 32) << 16) + rb;
+    unsigned char* bp_mine[3];  // its byte of the digit operand's rows rb, R + rb, 2 R + rb
+#pragma unroll
+    for (int b = 0; b < 3; b++)
+      bp_mine[b] = bp + (ti >> 4) * S::PITCH + (ti & 15) + ((b * R + rb) >> 3) * 128 + ((b * R + rb) & 7) * 16;
+    auto bar_group = [&]() { bar_named<128>(1 + grp); };
+    auto bar_all = [&]() { bar_named<S::COMPUTE>(3); };
     const uint32_t bq_a = smem_u32(bq), bp_a = smem_u32(bp), ring_a = smem_u32(ka_raw);
     constexpr uint32_t IDESC = tc_idesc(KA_TILE, S::N);
     int n = 0;  // tiles done by this CTA
@@ -273,7 +323,7 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
       const uint32_t a = ring_a + k * S::STAGE;
 #pragma unroll
       for (int i = 0; i < HD / 32; i++)
-        tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::NB * 16, S::NB * 16, 128, 0),
+        tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::PITCH, S::PITCH, 128, 0),
                    IDESC, i > 0);
       tc_commit(&sm.sbar);
     };
@@ -281,62 +331,69 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
       const KaPiece u = ka_piece(A, pre, t, end);
       const int last = ka_last(u);
       // ---- the block's queries as digits, and what its rows see ----
-      for (int r = warp; r < R; r += 4) {
-        const int node = r / A.g, h = u.kvh * A.g + r - node * A.g;
-        const bool on = node < u.nodes;
-        float x[E], amax = 0.0f, poison = 0.0f;
-        if (on) {
-          const float* src = A.q + ((size_t)(u.sp.r0 + u.j0 + node) * A.nh + h) * HD + lane * E;
+      constexpr int W = S::COMPUTE / 32;
+      float x[R / W][E];
+#pragma unroll
+      for (int i = 0; i < R / W; i++) {  // warp w: rows w, w + W, ...
+        const int r = warp + W * i;
+        const float* src = A.q + ((size_t)(u.sp.r0 + u.j0) * A.nh + u.kvh * A.g + sm.off[r]) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) x[i][e] = 0.0f;
+        if (sm.node[r] < u.nodes) {
           if constexpr (E == 4) {
             const float4 v = *reinterpret_cast<const float4*>(src);
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+            x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
           } else {
             const float2 v = *reinterpret_cast<const float2*>(src);
-            x[0] = v.x, x[1] = v.y;
+            x[i][0] = v.x, x[i][1] = v.y;
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; e++) x[e] = 0.0f;
         }
+      }
+      if (tid < R) {
+        int lim = 0;
+        if (sm.node[tid] < u.nodes) {
+          const int j = u.j0 + sm.node[tid];
+          const long long up_to = A.R.parent ? u.sp.start : (long long)u.sp.start + j + 1;
+          lim = kv8_parent(A.R, u.sp, j) == -2 ? -1 : (int)min(up_to, (long long)ka_cap(A.C));
+        }
+        sm.lim[tid] = lim;
+      }
+#pragma unroll
+      for (int i = 0; i < R / W; i++) {
+        const int r = warp + W * i;
+        float amax = 0.0f, poison = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          amax = fmaxf(amax, fabsf(x[e]));
-          poison = __fmaf_rn(x[e], 0.0f, poison);  // NaN for a NaN or an infinity
+          amax = fmaxf(amax, fabsf(x[i][e]));
+          poison = __fmaf_rn(x[i][e], 0.0f, poison);  // NaN for a NaN or an infinity
         }
         amax = warp_fmax(amax);
         const float inv = amax > 1e-30f ? __fdiv_rn(KA_FIX, amax) : 0.0f;  // below: the scores are zero
         uint32_t w[3] = {0, 0, 0};
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          const uint32_t d = to_digits((uint32_t)__float2int_rn(fminf(fmaxf(x[e] * inv, -KA_FIX), KA_FIX)));
+          const uint32_t d = to_digits((uint32_t)__float2int_rn(fminf(fmaxf(x[i][e] * inv, -KA_FIX), KA_FIX)));
 #pragma unroll
-          for (int i = 0; i < 3; i++) w[i] |= ((d >> (8 * i)) & 255u) << (8 * e);
+          for (int b = 0; b < 3; b++) w[b] |= ((d >> (8 * b)) & 255u) << (8 * e);
         }
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-          const int row = i * R + r, kb = lane * E;
-          unsigned char* d = bq + (kb >> 4) * (S::NB * 16) + (row >> 3) * 128 + (row & 7) * 16 + (kb & 15);
-          if constexpr (E == 4) *reinterpret_cast<uint32_t*>(d) = w[i];
-          else *reinterpret_cast<uint16_t*>(d) = (uint16_t)w[i];
+        for (int b = 0; b < 3; b++) {
+          const int row = b * R + r, kb = lane * E;
+          unsigned char* d = bq + (kb >> 4) * S::PITCH + (row >> 3) * 128 + (row & 7) * 16 + (kb & 15);
+          if constexpr (E == 4) *reinterpret_cast<uint32_t*>(d) = w[b];
+          else *reinterpret_cast<uint16_t*>(d) = (uint16_t)w[b];
         }
         const bool bad = __any_sync(0xffffffffu, poison != poison);
-        if (lane == 0) {
+        // never zero: the -infinity of a masked slot has to stay one
+        if (lane == 0)
           sm.qs[r] = bad ? __int_as_float(0x7fffffff)
-                         : (float)((double)amax / KA_FIX * (1.4426950408889634 / sqrt((double)HD)));
-          int lim = 0;
-          if (on) {
-            const int par = kv8_parent(A.R, u.sp, u.j0 + node);
-            const long long up_to = A.R.parent ? u.sp.start : (long long)u.sp.start + u.j0 + node + 1;
-            lim = par == -2 ? 0 : (int)min(up_to, (long long)ka_cap(A.C));
-          }
-          sm.lim[r] = lim;
-        }
+                         : fmaxf((float)((double)amax * (256.0 * 1.4426950408889634 / 8323072.0 / sqrt((double)HD))), 1e-37f);
       }
       fence_async_smem();
-      bar_compute();
-      float acc[R], l[R], m[R], c_run = 0.0f;
+      bar_all();
+      float acc[RT], l[RT], m[RT], c_run = 0.0f;
 #pragma unroll
-      for (int r = 0; r < R; r++) acc[r] = 0.0f, l[r] = 0.0f, m[r] = -INFINITY;
+      for (int r = 0; r < RT; r++) acc[r] = 0.0f, l[r] = 0.0f, m[r] = KA_NONE;
       if (tid == 0 && u.lo < last) {
         ka_wait(&sm.full[n % STAGES], (n / STAGES) & 1, &sm.fail);
         tc_fence_after();
@@ -344,10 +401,10 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
       }
       for (int tile = u.lo; tile < last; tile++, n++) {
         const int k = n % STAGES;
-        const int slot = tile * KA_TILE + tid;
+        const int slot = tile * KA_TILE + ti;
         unsigned char* st = ka_raw + k * S::STAGE;
         ka_wait(&sm.full[k], (n / STAGES) & 1, &sm.fail);  // the scales (the codes are the MMAs')
-        const float* sc = reinterpret_cast<const float*>(st + 2 * S::KBYTES + (tid >> 4) * 128) + (tid & 15);
+        const float* sc = reinterpret_cast<const float*>(st + 2 * S::KBYTES + (ti >> 4) * 128) + (ti & 15);
         const float ks = sc[0];
         float vs = sc[16];
         const uint32_t there = sm.pages[k];
@@ -359,7 +416,7 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
             // the path of each node, as bits of this tile
             if (tid < R) {
               uint32_t v[4] = {0, 0, 0, 0};
-              const int node = tid / A.g;
+              const int node = sm.node[tid];
               if (node < u.nodes) {
                 for (int at = u.j0 + node; at >= 0;) {
                   const int up = kv8_parent(A.R, u.sp, at);
@@ -377,80 +434,98 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
 #pragma unroll
               for (int i = 0; i < 4; i++) sm.vis[tid][i] = v[i];
             }
-            bar_compute();
+            bar_all();
           }
         }
         ka_wait(&sm.sbar, n & 1, &sm.fail);
         __syncwarp();
         tc_fence_after();
-        float s[R];
+        float s[RT];
 #pragma unroll
-        for (int r0 = 0; r0 < R; r0 += S::RC) {
+        for (int r0 = 0; r0 < RT; r0 += S::RC) {
           uint32_t d[3][S::RC];
           tmem_rows<S::RC>(tq + r0, R, d);
 #pragma unroll
-          for (int r = 0; r < S::RC; r++) s[r0 + r] = digits(d[0][r], d[1][r], d[2][r]) * sm.qs[r0 + r] * ks;
+          for (int r = 0; r < S::RC; r++) s[r0 + r] = ka_score(d[0][r], d[1][r], d[2][r]) * ks;
         }
         if (!whole) {
-          const bool in = (there >> (tid >> 4)) & 1u;
+          const bool in = (there >> (ti >> 4)) & 1u;
           const bool tree = A.R.parent && (tile + 1) * KA_TILE > u.sp.start;
           bool any = false;
 #pragma unroll
-          for (int r = 0; r < R; r++) {
-            bool see = slot < sm.lim[r];
-            if (tree) see = see || ((sm.vis[r][warp] >> lane) & 1u);
+          for (int r = 0; r < RT; r++) {
+            bool see = slot < sm.lim[rb + r];
+            if (tree) see = see || ((sm.vis[rb + r][quad] >> lane) & 1u);
             if (see && in) any = true;
             else s[r] = -INFINITY;
           }
           if (!any) vs = 0.0f;  // what lies in an unseen slot counts nowhere, not for the scales' maximum either
         }
-        // ---- the tile's maximum per row, and of the V scales ----
-        float mine = 0.0f;
+        // ---- the tile's maximum per row (a row's scale is left out until the exponent), and of the V scales ----
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-          const float v = warp_fmax(s[r]);
-          if (lane == r) mine = v;
+        for (int r = 0; r < RT; r += 4) {
+          const float4 v = make_float4(warp_fmax(s[r]), warp_fmax(s[r + 1]), warp_fmax(s[r + 2]), warp_fmax(s[r + 3]));
+          if (lane == 0) *reinterpret_cast<float4*>(&sm.wmax[quad][rb + r]) = v;
         }
-        if (lane < R) sm.wmax[lane][warp] = mine;
-        const float vfin = vs <= 3.402823466e38f ? vs : 0.0f;  // a NaN or infinite V scale: see `bad`
-        const float bad = __fmul_rn(vs, 0.0f);                 // NaN then, else 0
+        const float vfin = vs <= 3.402823466e38f ? vs : 0.0f;
         const float vm = warp_fmax(vfin);
-        if (lane == 0) sm.wsv[warp] = vm;
-        bar_compute();
-        c_run = fmaxf(fmaxf(c_run, fmaxf(sm.wsv[0], sm.wsv[1])), fmaxf(sm.wsv[2], sm.wsv[3]));
+        if (lane == 0) sm.wsv[grp][quad] = vm;
+        bar_group();
+        c_run = fmaxf(fmaxf(c_run, fmaxf(sm.wsv[grp][0], sm.wsv[grp][1])), fmaxf(sm.wsv[grp][2], sm.wsv[grp][3]));
         const float pf = c_run > 0.0f ? __fdiv_rn(vfin, c_run) * KA_FIX : 0.0f;
+        auto tile_max = [&](int r) {  // rows r .. r + 3
+          const float4 a = *reinterpret_cast<const float4*>(&sm.wmax[0][rb + r]), b = *reinterpret_cast<const float4*>(&sm.wmax[1][rb + r]);
+          const float4 c = *reinterpret_cast<const float4*>(&sm.wmax[2][rb + r]), d = *reinterpret_cast<const float4*>(&sm.wmax[3][rb + r]);
+          return make_float4(fmaxf(fmaxf(a.x, b.x), fmaxf(c.x, d.x)), fmaxf(fmaxf(a.y, b.y), fmaxf(c.y, d.y)),
+                             fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z)), fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w)));
+        };
+        bool grew = false;
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-          const float4 w4 = *reinterpret_cast<const float4*>(sm.wmax[r]);
-          const float mt = fmaxf(fmaxf(w4.x, w4.y), fmaxf(w4.z, w4.w));
-          if (mt > m[r]) {  // the same for every thread
-            const float al = m[r] == -INFINITY ? 0.0f : ex2(m[r] - mt);
-            acc[r] *= al;
-            l[r] *= al;
-            m[r] = mt;
+        for (int r = 0; r < RT; r += 4) {
+          const float4 v = tile_max(r);
+          grew = grew || v.x > m[r] || v.y > m[r + 1] || v.z > m[r + 2] || v.w > m[r + 3];
+        }
+        if (grew) {  // the same for every thread
+#pragma unroll
+          for (int r0 = 0; r0 < RT; r0 += 4) {
+            const float4 v = tile_max(r0);
+            const float mt[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int r = r0; r < r0 + 4; r++) {
+              const float mn = fmaxf(m[r], mt[r - r0]), al = ex2((m[r] - mn) * sm.qs[rb + r]);
+              acc[r] *= al;
+              l[r] *= al;
+              m[r] = mn;
+            }
           }
-          const float p = ex2(s[r] - (m[r] == -INFINITY ? 0.0f : m[r]));
-          const bool see = s[r] != -INFINITY;  // a NaN score is seen
-          l[r] += see ? p + bad : 0.0f;
+        }
+        if (__any_sync(0xffffffffu, vs != vfin)) {  // a NaN or infinite V scale poisons the rows that see the slot
+#pragma unroll
+          for (int r = 0; r < RT; r++)
+            if (vs != vfin && s[r] != -INFINITY) l[r] = __int_as_float(0x7fffffff);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          const float p = ex2(__fmul_rn(s[r] - m[r], sm.qs[rb + r]));
+          l[r] += p;
           // p * pf in [0, KA_FIX], rounded into the low bits of 2^23 + v
-          const uint32_t v = __float_as_uint(__fmaf_rn(see ? p : 0.0f, pf, 8388608.0f)) & 0x7fffffu;
-          const uint32_t d = to_digits(v);
+          const uint32_t d = to_digits(__float_as_uint(__fmaf_rn(p, pf, 8388608.0f)));
 #pragma unroll
           for (int i = 0; i < 3; i++) {
-            const int row = i * R + r;
-            bp_mine[(row >> 3) * 128 + (row & 7) * 16] = (unsigned char)(d >> (8 * i));
+            const int row = ((i * R) & 7) + r;  // rb is a multiple of 8
+            bp_mine[i][((row >> 3) * 128 + (row & 7) * 16) - ((i * R) & 7) * 16] = (unsigned char)(d >> (8 * i));
           }
         }
         fence_async_smem();
         tc_fence_before();
-        bar_compute();
+        bar_all();
         if (tid == 0) {
           tc_fence_after();
           const uint32_t a = ring_a + k * S::STAGE + S::KBYTES;
 #pragma unroll
           for (int i = 0; i < KA_TILE / 32; i++)
             tc_mma_acc(tm + S::COL_O, tc_desc(a + i * 32 * HD, 16 * HD, 128, 0),
-                       tc_desc(bp_a + i * 2 * S::NB * 16, S::NB * 16, 128, 0), IDESC, i > 0);
+                       tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC, i > 0);
           tc_commit(&sm.obar);
           if (tile + 1 < last) {  // the next tile's scores meanwhile
             ka_wait(&sm.full[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
@@ -462,39 +537,35 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
         __syncwarp();
         tc_fence_after();
         if (tid == 0) mbar_arrive(&sm.empty[k]);  // V was read, K and the scales long before
-        const float of = c_run * (1.0f / KA_FIX);
+        const float of = c_run * (1.0f / KA_FIX), of256 = of * 256.0f;
 #pragma unroll
-        for (int r0 = 0; r0 < R; r0 += S::RC) {
+        for (int r0 = 0; r0 < RT; r0 += S::RC) {
           uint32_t d[3][S::RC];
           tmem_rows<S::RC>(tq + S::COL_O + r0, R, d);
 #pragma unroll
-          for (int r = 0; r < S::RC; r++) acc[r0 + r] = __fmaf_rn(digits(d[0][r], d[1][r], d[2][r]), of, acc[r0 + r]);
+          for (int r = 0; r < S::RC; r++) acc[r0 + r] = ka_add(d[0][r], d[1][r], d[2][r], of, of256, acc[r0 + r]);
         }
         tc_fence_before();
       }
       // ---- the unit's (or its share's) end ----
-#pragma unroll
-      for (int r = 0; r < R; r++) {
-        const float v = warp_sum(l[r]);
-        if (lane == 0) sm.wsum[r][warp] = v;
-      }
-      bar_compute();
+      const float mine = warp_sums(l);
+      if (lane < RT) sm.wsum[quad][rb + lane] = mine;
+      bar_group();
       const bool from0 = u.lo == 0, to_end = u.hi == u.tiles;
       float* part = A.part + ((size_t)cta * 2 + (from0 ? 1 : 0)) * R * (HD + 2);
+      float* out = A.out + ((size_t)(u.sp.r0 + u.j0) * A.nh + u.kvh * A.g) * HD + ti;
 #pragma unroll
-      for (int r = 0; r < R; r++) {
-        const int node = r / A.g, h = u.kvh * A.g + r - node * A.g;
-        const float4 w4 = *reinterpret_cast<const float4*>(sm.wsum[r]);
-        const bool dead = kv8_parent(A.R, u.sp, u.j0 + min(node, u.nodes - 1)) == -2;
-        const float tot = dead ? 0.0f : (w4.x + w4.y) + (w4.z + w4.w);
+      for (int r = 0; r < RT; r++) {
+        const int row = rb + r;
+        float tot = (sm.wsum[0][row] + sm.wsum[1][row]) + (sm.wsum[2][row] + sm.wsum[3][row]);
+        if (sm.lim[row] < 0) tot = 0.0f;
         if (from0 && to_end) {
-          if (node < u.nodes && tid < HD)
-            A.out[((size_t)(u.sp.r0 + u.j0 + node) * A.nh + h) * HD + tid] = tot == 0.0f ? 0.0f : __fdiv_rn(acc[r], tot);
+          if (sm.node[row] < u.nodes && ti < HD) out[sm.off[row] * HD] = tot == 0.0f ? 0.0f : __fdiv_rn(acc[r], tot);
         } else {
-          if (tid < HD) part[r * HD + tid] = acc[r];
-          if (tid == 0) {
-            part[R * HD + r] = m[r];
-            part[R * HD + R + r] = tot;
+          if (ti < HD) part[row * HD + ti] = acc[r];
+          if (ti == 0) {
+            part[R * HD + row] = m[r] * sm.qs[row];
+            part[R * HD + R + row] = tot;
           }
         }
       }
@@ -503,37 +574,42 @@ __global__ void __launch_bounds__(KA_THREADS, R == 32 ? 2 : 3) k_kv8_attn(const 
         const int lt = u.u0 + u.tiles - 1;
         A.head[cta] = make_int4(u.sp.r0 + u.j0, u.kvh, u.nodes, (int)((((long long)lt + 1) * G - 1) / T));
       }
-      bar_compute();
+      bar_all();
       t = u.u0 + u.hi;
     }
   }
   // ---- wind-down: every MMA was waited for (bounded) by its tile; free the columns ----
   tc_fence_before();
   __syncthreads();
-  if (warp == KA_COMPUTE / 32)
+  if (warp == COPY)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(S::COLS));
   if (tid == 0 && sm.fail) kv8_flag(A.R.err, HG_ERR_TIMEOUT);
 }
 
 // The partial results of a unit whose tiles lie in several CTAs, added up in tile order: one CTA per
-// first share and row.
+// first share and four rows.
 template <int HD, int R>
-__global__ void __launch_bounds__(HD) k_kv8_join(const __grid_constant__ KaArgs A) {
+__global__ void __launch_bounds__(4 * HD) k_kv8_join(const __grid_constant__ KaArgs A) {
   pdl_wait();
   pdl_trigger();
-  const int c0 = blockIdx.x, r = blockIdx.y;
+  const int c0 = blockIdx.x, r = blockIdx.y * 4 + threadIdx.y;
   const int4 h = A.head[c0];
   if (h.x < 0) return;
   const int node = r / A.g;
   if (node >= h.z) return;
   constexpr int P = R * (HD + 2);
-  auto part = [&](int c) { return A.part + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * P; };
-  float mx = -INFINITY;
-  for (int c = c0; c <= h.w; c++) mx = fmaxf(mx, part(c)[R * HD + r]);
-  float o = 0.0f, tot = 0.0f;
-  for (int c = c0; c <= h.w; c++) {
-    const float* p = part(c);
-    const float m = p[R * HD + r], f = m == -INFINITY ? 0.0f : ex2(m - mx);
+  const float* first = A.part + ((size_t)c0 * 2 + 1) * P;       // the first share's
+  const float* next = A.part + (size_t)(c0 + 1) * 2 * P;        // and the following CTAs'
+  const int n = h.w - c0;
+  float mx = first[R * HD + r];
+#pragma unroll 8
+  for (int i = 0; i < n; i++) mx = fmaxf(mx, next[(size_t)i * 2 * P + R * HD + r]);
+  const float f0 = ex2(first[R * HD + r] - mx);
+  float o = first[r * HD + threadIdx.x] * f0, tot = first[R * HD + R + r] * f0;
+#pragma unroll 8
+  for (int i = 0; i < n; i++) {
+    const float* p = next + (size_t)i * 2 * P;
+    const float f = ex2(p[R * HD + r] - mx);
     o = __fmaf_rn(p[r * HD + threadIdx.x], f, o);
     tot = __fmaf_rn(p[R * HD + R + r], f, tot);
   }
@@ -576,7 +652,7 @@ void launch(KaArgs& A, int device, cudaStream_t st) {
   const int per_sm = (int)std::min<size_t>(std::min(3, 512 / S::COLS), (228 * 1024) / (smem + 1024));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(KA_SMS * per_sm);
-  cfg.blockDim = dim3(KA_THREADS);
+  cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -585,8 +661,8 @@ void launch(KaArgs& A, int device, cudaStream_t st) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_attn<HD, R>, A));
-  cfg.gridDim = dim3(KA_SMS * per_sm, R);
-  cfg.blockDim = dim3(HD);
+  cfg.gridDim = dim3(KA_SMS * per_sm, R / 4);
+  cfg.blockDim = dim3(HD, 4);
   cfg.dynamicSmemBytes = 0;
   kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_join<HD, R>, A));
 }

@@ -46,9 +46,11 @@ struct KaShape {
   // bytes between 16-byte columns of the digit operands: 16 more than the rows take, so that the two
   // columns that a warp's 32 slots lie in use different banks
   static constexpr int PITCH = NB * 16 + 16;
-  static constexpr int KBYTES = KA_TILE * HD, STAGE = 2 * KBYTES + KA_PAGES * 128;
+  // the rings: V tiles, then K tiles with the scales of both (what a 64-dim V operand reads past its
+  // tile, for M = 128, is the next tile)
+  static constexpr int VSTAGE = KA_TILE * HD, KSTAGE = VSTAGE + KA_PAGES * 128;
   static constexpr int STAGES = HD == 128 ? 2 : 4;
-  static constexpr int OFF_BQ = STAGES * STAGE, OFF_BP = OFF_BQ + PITCH * (HD / 16),
+  static constexpr int OFF_K = STAGES * VSTAGE, OFF_BQ = OFF_K + STAGES * KSTAGE, OFF_BP = OFF_BQ + PITCH * (HD / 16),
                        OFF_SMALL = OFF_BP + PITCH * (KA_TILE / 16);
   // tensor-memory columns: S at 0, O behind it; a power of two of at least 32
   static constexpr int COL_O = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;
@@ -62,9 +64,10 @@ struct KaShape {
 
 template <int R>
 struct KaSmall {
-  uint64_t full[4], empty[4], sbar, obar;
+  uint64_t full_k[4], empty_k[4], full_v[4], empty_v[4], sbar, obar;
   float wmax[4][R];          // per warp maxima of a tile's scores
   float wsum[4][R];          // per warp sums at a unit's end
+  float m[2][R];             // running maxima, by the tile's parity
   float qs[R];               // row r: 256 log2(e) / sqrt(hd) * q scale
   int lim[R];                // row r sees the slots below, and the tree slots of `vis`; -1: padding
   int node[R], off[R];       // row r's node within its block, its q head's place behind the block's first
@@ -85,6 +88,31 @@ struct KaArgs {
   int4* head;      // [CTA][2] of the joins: {sequence, kv head * 65536.. (see k_kv8_join)}
 };
 
+// Two rows' f32 values side by side: one instruction for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -113,8 +141,9 @@ __device__ __forceinline__ void mbar_arrive_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ float ka_score(uint32_t d0, uint32_t d1, uint32_t d2) {
   return __int2float_rn((int)((d2 << 8) + d1) + ((int)d0 >> 8));
 }
-__device__ __forceinline__ float ka_add(uint32_t d0, uint32_t d1, uint32_t d2, float f, float f256, float acc) {
-  return __fmaf_rn(__int2float_rn((int)((d2 << 8) + d1)), f256, __fmaf_rn(tc_isum(d0), f, acc));
+__device__ __forceinline__ f32x2 ka_add(const uint32_t (&d)[3][2], f32x2 f, f32x2 f256, f32x2 acc) {
+  const f32x2 hi = pack2(__int2float_rn((int)((d[2][0] << 8) + d[1][0])), __int2float_rn((int)((d[2][1] << 8) + d[1][1])));
+  return fma2(hi, f256, fma2(pack2(__int2float_rn((int)d[0][0]), __int2float_rn((int)d[0][1])), f, acc));
 }
 // Sums over the warp of R values per lane: lane i < R gets value i's.
 template <int R>
@@ -196,11 +225,20 @@ __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre
 // Tiles from here on show nothing to the block's rows.
 __device__ __forceinline__ int ka_last(const KaPiece& u) { return min(u.hi, (u.seen + KA_TILE - 1) / KA_TILE); }
 
-__device__ __forceinline__ bool ka_wait(uint64_t* bar, uint32_t parity, int* fail) {
-  if (*reinterpret_cast<volatile int*>(fail)) return false;
-  if (mbar_wait(bar, parity)) return true;
+// A bounded wait; after the first that gave up, every other gives up soon.
+__device__ __forceinline__ void ka_wait(uint64_t* bar, uint32_t parity, int* fail) {
+  const uint32_t a = smem_u32(bar);
+  for (long long i = 1; i < TC_SPIN_LIMIT; i++) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return;
+    if (i % 1024 == 0 && *reinterpret_cast<volatile int*>(fail)) return;
+  }
   *reinterpret_cast<volatile int*>(fail) = 1;
-  return false;
 }
 
 template <int HD, int R>
@@ -229,8 +267,10 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   if (tid == 0) {
     pre[0] = 0;
     for (int k = 0; k < STAGES; k++) {
-      mbar_init(&sm.full[k], KA_PAGES);
-      mbar_init(&sm.empty[k], 1);
+      mbar_init(&sm.full_k[k], KA_PAGES);
+      mbar_init(&sm.full_v[k], KA_PAGES);
+      mbar_init(&sm.empty_k[k], 1);
+      mbar_init(&sm.empty_v[k], 1);
     }
     mbar_init(&sm.sbar, 1);
     mbar_init(&sm.obar, 1);
@@ -285,26 +325,39 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       const uint8_t* src = page_of(u.lo);
       for (int tile = u.lo; tile < last; tile++, n++) {
         const int k = n % STAGES;
-        if (n >= STAGES) ka_wait(&sm.empty[k], (n / STAGES - 1) & 1, &sm.fail);
+        const uint32_t past = (n / STAGES - 1) & 1;
+        if (n >= STAGES) ka_wait(&sm.empty_k[k], past, &sm.fail);
         const uint32_t there = __ballot_sync(0xffffffffu, src != nullptr);
         if (lane == 0) sm.pages[k] = there;
         __syncwarp();
         if (lane < KA_PAGES) {
-          unsigned char* st = ka_raw + k * S::STAGE;
           if (src) {
-            mbar_arrive_tx(&sm.full[k], kv8_block_bytes(HD));
-            bulk_copy(st + lane * 16 * HD, src, 16 * HD, &sm.full[k]);
-            bulk_copy(st + S::KBYTES + lane * 16 * HD, src + 16 * HD, 16 * HD, &sm.full[k]);
-            bulk_copy(st + 2 * S::KBYTES + lane * 128, src + 32 * HD, 128, &sm.full[k]);
+            unsigned char* st = ka_raw + S::OFF_K + k * S::KSTAGE;
+            mbar_arrive_tx(&sm.full_k[k], 16 * HD + 128);
+            bulk_copy(st + lane * 16 * HD, src, 16 * HD, &sm.full_k[k]);
+            bulk_copy(st + S::VSTAGE + lane * 128, src + 32 * HD, 128, &sm.full_k[k]);
           } else {
-            mbar_arrive(&sm.full[k]);
+            mbar_arrive(&sm.full_k[k]);
           }
         }
-        src = page_of(tile + 1);
+        const uint8_t* next = page_of(tile + 1);
+        if (n >= STAGES) ka_wait(&sm.empty_v[k], past, &sm.fail);
+        if (lane < KA_PAGES) {
+          if (src) {
+            mbar_arrive_tx(&sm.full_v[k], 16 * HD);
+            bulk_copy(ka_raw + k * S::VSTAGE + lane * 16 * HD, src + 16 * HD, 16 * HD, &sm.full_v[k]);
+          } else {
+            mbar_arrive(&sm.full_v[k]);
+          }
+        }
+        src = next;
       }
       t = u.u0 + u.hi;
     }
-    for (int i = max(0, n - STAGES); i < n; i++) mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1);
+    for (int i = max(0, n - STAGES); i < n; i++) {
+      mbar_wait(&sm.full_k[i % STAGES], (i / STAGES) & 1);
+      mbar_wait(&sm.full_v[i % STAGES], (i / STAGES) & 1);
+    }
   } else {
     // =================== compute warps ===================
     // this thread: slot / dim ti of the tile, rows rb .. rb + RT - 1
@@ -314,13 +367,16 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
 #pragma unroll
     for (int b = 0; b < 3; b++)
       bp_mine[b] = bp + (ti >> 4) * S::PITCH + (ti & 15) + ((b * R + rb) >> 3) * 128 + ((b * R + rb) & 7) * 16;
-    auto bar_group = [&]() { bar_named<128>(1 + grp); };
-    auto bar_all = [&]() { bar_named<S::COMPUTE>(3); };
+    auto bar_all = [&]() { bar_named<S::COMPUTE>(1); };
+    auto bar_group = [&]() {
+      if constexpr (S::GROUPS == 1) bar_all();
+      else bar_named<128>(2 + grp);
+    };
     const uint32_t bq_a = smem_u32(bq), bp_a = smem_u32(bp), ring_a = smem_u32(ka_raw);
     constexpr uint32_t IDESC = tc_idesc(KA_TILE, S::N);
     int n = 0;  // tiles done by this CTA
     auto issue_scores = [&](int k) {  // thread 0: S = K . q digits
-      const uint32_t a = ring_a + k * S::STAGE;
+      const uint32_t a = ring_a + S::OFF_K + k * S::KSTAGE;
 #pragma unroll
       for (int i = 0; i < HD / 32; i++)
         tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::PITCH, S::PITCH, 128, 0),
@@ -357,6 +413,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           lim = kv8_parent(A.R, u.sp, j) == -2 ? -1 : (int)min(up_to, (long long)ka_cap(A.C));
         }
         sm.lim[tid] = lim;
+        sm.m[0][tid] = sm.m[1][tid] = KA_NONE;
       }
 #pragma unroll
       for (int i = 0; i < R / W; i++) {
@@ -391,164 +448,201 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       }
       fence_async_smem();
       bar_all();
-      float acc[RT], l[RT], m[RT], c_run = 0.0f;
+      f32x2 acc[RT / 2], l[RT / 2];
+      float c_run = 0.0f, of = 0.0f;
 #pragma unroll
-      for (int r = 0; r < RT; r++) acc[r] = 0.0f, l[r] = 0.0f, m[r] = KA_NONE;
+      for (int r = 0; r < RT / 2; r++) acc[r] = l[r] = 0ull;
+      // the sums over the dims that the MMAs of tile n - 1 left in tensor memory
+      auto add_out = [&](int n_of) {
+        ka_wait(&sm.obar, n_of & 1, &sm.fail);
+        __syncwarp();
+        tc_fence_after();
+        if (tid == 0) mbar_arrive(&sm.empty_v[n_of % STAGES]);
+        const f32x2 f = pack2(of, of), f256 = pack2(of * 256.0f, of * 256.0f);
+#pragma unroll
+        for (int r0 = 0; r0 < RT; r0 += S::RC) {
+          uint32_t d[3][S::RC];
+          tmem_rows<S::RC>(tq + S::COL_O + r0, R, d);
+#pragma unroll
+          for (int r = 0; r < S::RC; r += 2) {
+            const uint32_t e[3][2] = {{d[0][r], d[0][r + 1]}, {d[1][r], d[1][r + 1]}, {d[2][r], d[2][r + 1]}};
+            acc[(r0 + r) / 2] = ka_add(e, f, f256, acc[(r0 + r) / 2]);
+          }
+        }
+        tc_fence_before();
+      };
       if (tid == 0 && u.lo < last) {
-        ka_wait(&sm.full[n % STAGES], (n / STAGES) & 1, &sm.fail);
+        ka_wait(&sm.full_k[n % STAGES], (n / STAGES) & 1, &sm.fail);
         tc_fence_after();
         issue_scores(n % STAGES);
       }
       for (int tile = u.lo; tile < last; tile++, n++) {
         const int k = n % STAGES;
         const int slot = tile * KA_TILE + ti;
-        unsigned char* st = ka_raw + k * S::STAGE;
-        ka_wait(&sm.full[k], (n / STAGES) & 1, &sm.fail);  // the scales (the codes are the MMAs')
-        const float* sc = reinterpret_cast<const float*>(st + 2 * S::KBYTES + (ti >> 4) * 128) + (ti & 15);
+        ka_wait(&sm.full_k[k], (n / STAGES) & 1, &sm.fail);  // the scales (the codes are the MMAs')
+        const float* sc =
+            reinterpret_cast<const float*>(ka_raw + S::OFF_K + k * S::KSTAGE + S::VSTAGE + (ti >> 4) * 128) + (ti & 15);
         const float ks = sc[0];
         float vs = sc[16];
         const uint32_t there = sm.pages[k];
         // every slot is context of every row and its page is there: nothing to mask
         const bool whole = there == (1u << KA_PAGES) - 1 && (tile + 1) * KA_TILE <= u.sp.start;
-        if (!whole) {
-          const bool tree = A.R.parent && (tile + 1) * KA_TILE > u.sp.start;
-          if (tree) {
-            // the path of each node, as bits of this tile
-            if (tid < R) {
-              uint32_t v[4] = {0, 0, 0, 0};
-              const int node = sm.node[tid];
-              if (node < u.nodes) {
-                for (int at = u.j0 + node; at >= 0;) {
-                  const int up = kv8_parent(A.R, u.sp, at);
-                  if (up == -2) break;
-                  const long long b = (long long)u.sp.start + at - (long long)tile * KA_TILE;
-                  if (b < 0) break;  // ancestors lie below
-                  if (b < KA_TILE) {
+        const bool tree = A.R.parent && (tile + 1) * KA_TILE > u.sp.start;
+        if (tree) {
+          // the path of each node, as bits of this tile
+          if (tid < R) {
+            uint32_t v[4] = {0, 0, 0, 0};
+            const int node = sm.node[tid];
+            if (node < u.nodes) {
+              for (int at = u.j0 + node; at >= 0;) {
+                const int up = kv8_parent(A.R, u.sp, at);
+                if (up == -2) break;
+                const long long b = (long long)u.sp.start + at - (long long)tile * KA_TILE;
+                if (b < 0) break;  // ancestors lie below
+                if (b < KA_TILE) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                      if ((b >> 5) == i) v[i] |= 1u << (b & 31);
-                  }
-                  at = up;
+                  for (int i = 0; i < 4; i++)
+                    if ((b >> 5) == i) v[i] |= 1u << (b & 31);
                 }
+                at = up;
               }
-#pragma unroll
-              for (int i = 0; i < 4; i++) sm.vis[tid][i] = v[i];
             }
-            bar_all();
+#pragma unroll
+            for (int i = 0; i < 4; i++) sm.vis[tid][i] = v[i];
           }
+          bar_all();
         }
         ka_wait(&sm.sbar, n & 1, &sm.fail);
         __syncwarp();
         tc_fence_after();
-        float s[RT];
+        f32x2 s[RT / 2];
+        const f32x2 ks2 = pack2(ks, ks);
 #pragma unroll
         for (int r0 = 0; r0 < RT; r0 += S::RC) {
           uint32_t d[3][S::RC];
           tmem_rows<S::RC>(tq + r0, R, d);
 #pragma unroll
-          for (int r = 0; r < S::RC; r++) s[r0 + r] = ka_score(d[0][r], d[1][r], d[2][r]) * ks;
+          for (int r = 0; r < S::RC; r += 2)
+            s[(r0 + r) / 2] = mul2(pack2(ka_score(d[0][r], d[1][r], d[2][r]), ka_score(d[0][r + 1], d[1][r + 1], d[2][r + 1])), ks2);
         }
         if (!whole) {
           const bool in = (there >> (ti >> 4)) & 1u;
-          const bool tree = A.R.parent && (tile + 1) * KA_TILE > u.sp.start;
           bool any = false;
 #pragma unroll
-          for (int r = 0; r < RT; r++) {
-            bool see = slot < sm.lim[rb + r];
-            if (tree) see = see || ((sm.vis[rb + r][quad] >> lane) & 1u);
-            if (see && in) any = true;
-            else s[r] = -INFINITY;
+          for (int r = 0; r < RT; r += 2) {
+            float x[2];
+            unpack2(s[r / 2], x[0], x[1]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              bool see = slot < sm.lim[rb + r + i];
+              if (tree) see = see || ((sm.vis[rb + r + i][quad] >> lane) & 1u);
+              if (see && in) any = true;
+              else x[i] = -INFINITY;
+            }
+            s[r / 2] = pack2(x[0], x[1]);
           }
           if (!any) vs = 0.0f;  // what lies in an unseen slot counts nowhere, not for the scales' maximum either
         }
         // ---- the tile's maximum per row (a row's scale is left out until the exponent), and of the V scales ----
 #pragma unroll
         for (int r = 0; r < RT; r += 4) {
-          const float4 v = make_float4(warp_fmax(s[r]), warp_fmax(s[r + 1]), warp_fmax(s[r + 2]), warp_fmax(s[r + 3]));
+          float x[4];
+          unpack2(s[r / 2], x[0], x[1]);
+          unpack2(s[r / 2 + 1], x[2], x[3]);
+          const float4 v = make_float4(warp_fmax(x[0]), warp_fmax(x[1]), warp_fmax(x[2]), warp_fmax(x[3]));
           if (lane == 0) *reinterpret_cast<float4*>(&sm.wmax[quad][rb + r]) = v;
         }
         const float vfin = vs <= 3.402823466e38f ? vs : 0.0f;
         const float vm = warp_fmax(vfin);
         if (lane == 0) sm.wsv[grp][quad] = vm;
+        if (tile > u.lo) add_out(n - 1);  // the previous tile's sums, while the others get here
         bar_group();
         c_run = fmaxf(fmaxf(c_run, fmaxf(sm.wsv[grp][0], sm.wsv[grp][1])), fmaxf(sm.wsv[grp][2], sm.wsv[grp][3]));
         const float pf = c_run > 0.0f ? __fdiv_rn(vfin, c_run) * KA_FIX : 0.0f;
-        auto tile_max = [&](int r) {  // rows r .. r + 3
-          const float4 a = *reinterpret_cast<const float4*>(&sm.wmax[0][rb + r]), b = *reinterpret_cast<const float4*>(&sm.wmax[1][rb + r]);
-          const float4 c = *reinterpret_cast<const float4*>(&sm.wmax[2][rb + r]), d = *reinterpret_cast<const float4*>(&sm.wmax[3][rb + r]);
-          return make_float4(fmaxf(fmaxf(a.x, b.x), fmaxf(c.x, d.x)), fmaxf(fmaxf(a.y, b.y), fmaxf(c.y, d.y)),
-                             fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z)), fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w)));
-        };
+        const int now = n & 1;
+        float m[RT];
         bool grew = false;
 #pragma unroll
         for (int r = 0; r < RT; r += 4) {
-          const float4 v = tile_max(r);
-          grew = grew || v.x > m[r] || v.y > m[r + 1] || v.z > m[r + 2] || v.w > m[r + 3];
+          const float4 a = *reinterpret_cast<const float4*>(&sm.wmax[0][rb + r]), b = *reinterpret_cast<const float4*>(&sm.wmax[1][rb + r]);
+          const float4 c = *reinterpret_cast<const float4*>(&sm.wmax[2][rb + r]), d = *reinterpret_cast<const float4*>(&sm.wmax[3][rb + r]);
+          const float4 o = *reinterpret_cast<const float4*>(&sm.m[now ^ 1][rb + r]);
+          m[r] = fmaxf(fmaxf(fmaxf(a.x, b.x), fmaxf(c.x, d.x)), o.x);
+          m[r + 1] = fmaxf(fmaxf(fmaxf(a.y, b.y), fmaxf(c.y, d.y)), o.y);
+          m[r + 2] = fmaxf(fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z)), o.z);
+          m[r + 3] = fmaxf(fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w)), o.w);
+          if (ti == 0) *reinterpret_cast<float4*>(&sm.m[now][rb + r]) = make_float4(m[r], m[r + 1], m[r + 2], m[r + 3]);
+          grew = grew || m[r] > o.x || m[r + 1] > o.y || m[r + 2] > o.z || m[r + 3] > o.w;
         }
-        if (grew) {  // the same for every thread
+        if (grew) {  // the same for every thread of the group
 #pragma unroll
-          for (int r0 = 0; r0 < RT; r0 += 4) {
-            const float4 v = tile_max(r0);
-            const float mt[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int r = r0; r < r0 + 4; r++) {
-              const float mn = fmaxf(m[r], mt[r - r0]), al = ex2((m[r] - mn) * sm.qs[rb + r]);
-              acc[r] *= al;
-              l[r] *= al;
-              m[r] = mn;
-            }
+          for (int r = 0; r < RT; r += 2) {
+            const float2 o = *reinterpret_cast<const float2*>(&sm.m[now ^ 1][rb + r]);
+            const float2 q2 = *reinterpret_cast<const float2*>(&sm.qs[rb + r]);
+            const f32x2 al = pack2(ex2((o.x - m[r]) * q2.x), ex2((o.y - m[r + 1]) * q2.y));
+            acc[r / 2] = mul2(acc[r / 2], al);
+            l[r / 2] = mul2(l[r / 2], al);
           }
         }
         if (__any_sync(0xffffffffu, vs != vfin)) {  // a NaN or infinite V scale poisons the rows that see the slot
+          const float bad = vs != vfin ? __int_as_float(0x7fffffff) : 0.0f;
 #pragma unroll
-          for (int r = 0; r < RT; r++)
-            if (vs != vfin && s[r] != -INFINITY) l[r] = __int_as_float(0x7fffffff);
-        }
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-          const float p = ex2(__fmul_rn(s[r] - m[r], sm.qs[rb + r]));
-          l[r] += p;
-          // p * pf in [0, KA_FIX], rounded into the low bits of 2^23 + v
-          const uint32_t d = to_digits(__float_as_uint(__fmaf_rn(p, pf, 8388608.0f)));
-#pragma unroll
-          for (int i = 0; i < 3; i++) {
-            const int row = ((i * R) & 7) + r;  // rb is a multiple of 8
-            bp_mine[i][((row >> 3) * 128 + (row & 7) * 16) - ((i * R) & 7) * 16] = (unsigned char)(d >> (8 * i));
+          for (int r = 0; r < RT; r += 2) {
+            float x[2];
+            unpack2(s[r / 2], x[0], x[1]);
+            l[r / 2] = add2(l[r / 2], pack2(x[0] != -INFINITY ? bad : 0.0f, x[1] != -INFINITY ? bad : 0.0f));
           }
         }
+        const f32x2 pf2 = pack2(pf, pf), minus1 = pack2(-1.0f, -1.0f), big = pack2(8388608.0f, 8388608.0f);
+#pragma unroll
+        for (int r = 0; r < RT; r += 2) {
+          const float2 q2 = *reinterpret_cast<const float2*>(&sm.qs[rb + r]);
+          float x[2];
+          unpack2(mul2(fma2(pack2(m[r], m[r + 1]), minus1, s[r / 2]), pack2(q2.x, q2.y)), x[0], x[1]);
+          const f32x2 p = pack2(ex2(x[0]), ex2(x[1]));
+          l[r / 2] = add2(l[r / 2], p);
+          // p * pf in [0, KA_FIX], rounded into the low bits of 2^23 + v
+          unpack2(fma2(p, pf2, big), x[0], x[1]);
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const uint32_t d = to_digits(__float_as_uint(x[i]));
+#pragma unroll
+            for (int b = 0; b < 3; b++) {
+              const int row = ((b * R) & 7) + r + i;  // rb is a multiple of 8
+              bp_mine[b][((row >> 3) * 128 + (row & 7) * 16) - ((b * R) & 7) * 16] = (unsigned char)(d >> (8 * b));
+            }
+          }
+        }
+        of = c_run * (1.0f / KA_FIX);
         fence_async_smem();
         tc_fence_before();
         bar_all();
         if (tid == 0) {
+          mbar_arrive(&sm.empty_k[k]);  // its scores are done, and every thread has its scales
+          ka_wait(&sm.full_v[k], (n / STAGES) & 1, &sm.fail);
           tc_fence_after();
-          const uint32_t a = ring_a + k * S::STAGE + S::KBYTES;
+          const uint32_t a = ring_a + k * S::VSTAGE;
 #pragma unroll
           for (int i = 0; i < KA_TILE / 32; i++)
             tc_mma_acc(tm + S::COL_O, tc_desc(a + i * 32 * HD, 16 * HD, 128, 0),
                        tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC, i > 0);
           tc_commit(&sm.obar);
           if (tile + 1 < last) {  // the next tile's scores meanwhile
-            ka_wait(&sm.full[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
+            ka_wait(&sm.full_k[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
             issue_scores((n + 1) % STAGES);
           }
         }
         __syncwarp();
-        ka_wait(&sm.obar, n & 1, &sm.fail);
-        __syncwarp();
-        tc_fence_after();
-        if (tid == 0) mbar_arrive(&sm.empty[k]);  // V was read, K and the scales long before
-        const float of = c_run * (1.0f / KA_FIX), of256 = of * 256.0f;
-#pragma unroll
-        for (int r0 = 0; r0 < RT; r0 += S::RC) {
-          uint32_t d[3][S::RC];
-          tmem_rows<S::RC>(tq + S::COL_O + r0, R, d);
-#pragma unroll
-          for (int r = 0; r < S::RC; r++) acc[r0 + r] = ka_add(d[0][r], d[1][r], d[2][r], of, of256, acc[r0 + r]);
-        }
-        tc_fence_before();
       }
+      if (u.lo < last) add_out(n - 1);
       // ---- the unit's (or its share's) end ----
-      const float mine = warp_sums(l);
+      float ls[RT], sums[RT];
+#pragma unroll
+      for (int r = 0; r < RT; r += 2) {
+        unpack2(l[r / 2], ls[r], ls[r + 1]);
+        unpack2(acc[r / 2], sums[r], sums[r + 1]);
+      }
+      const float mine = warp_sums(ls);
       if (lane < RT) sm.wsum[quad][rb + lane] = mine;
       bar_group();
       const bool from0 = u.lo == 0, to_end = u.hi == u.tiles;
@@ -560,11 +654,11 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         float tot = (sm.wsum[0][row] + sm.wsum[1][row]) + (sm.wsum[2][row] + sm.wsum[3][row]);
         if (sm.lim[row] < 0) tot = 0.0f;
         if (from0 && to_end) {
-          if (sm.node[row] < u.nodes && ti < HD) out[sm.off[row] * HD] = tot == 0.0f ? 0.0f : __fdiv_rn(acc[r], tot);
+          if (sm.node[row] < u.nodes && ti < HD) out[sm.off[row] * HD] = tot == 0.0f ? 0.0f : __fdiv_rn(sums[r], tot);
         } else {
-          if (ti < HD) part[row * HD + ti] = acc[r];
+          if (ti < HD) part[row * HD + ti] = sums[r];
           if (ti == 0) {
-            part[R * HD + row] = m[r] * sm.qs[row];
+            part[R * HD + row] = sm.m[(n + 1) & 1][row] * sm.qs[row];
             part[R * HD + R + row] = tot;
           }
         }

@@ -25,6 +25,7 @@
 // (bounded again), frees its tensor memory and returns.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "hg_kv8.cuh"
 #include "hg_tc.cuh"
@@ -57,9 +58,9 @@ struct KaShape {
   static constexpr int COLS = 2 * COL_O;
   // Compute warps: groups of 128 threads, one slot (S) or dim (O) per thread and RT rows per group; and
   // the copy warp.
-  static constexpr int GROUPS = R > 16 ? R / 16 : 1, RT = R / GROUPS, COMPUTE = 128 * GROUPS, THREADS = COMPUTE + 32;
+  static constexpr int GROUPS = R > 8 ? 2 : 1, RT = R / GROUPS, COMPUTE = 128 * GROUPS, THREADS = COMPUTE + 32;
   static constexpr int RC = RT < 8 ? RT : 8;  // rows per tensor-memory read
-  static constexpr int PER_SM = R > 16 ? 2 : 3;
+  static constexpr int PER_SM = R > 8 ? 2 : 3;
 };
 
 template <int R>
@@ -72,7 +73,7 @@ struct KaSmall {
   int lim[R];                // row r sees the slots below, and the tree slots of `vis`; -1: padding
   int node[R], off[R];       // row r's node within its block, its q head's place behind the block's first
   uint32_t vis[R][4];        // slots of the current tile that row r's path holds
-  float wsv[R > 16 ? R / 16 : 1][4];
+  float wsv[2][4];
   uint32_t pages[4];         // per stage: which of the tile's pages are there
   uint32_t tmem;
   int fail;
@@ -189,7 +190,7 @@ __device__ __forceinline__ void tmem_rows(uint32_t t, uint32_t stride, uint32_t 
 
 // A run of tiles of one unit, as both the copy warp and the compute warps walk it.
 struct KaPiece {
-  int s, kvh, blk, u0, tiles, lo, hi;  // unit's first tile on the line and tile count; this CTA's share
+  int s, kvh, blk, u0, next, tiles, lo, hi;  // the unit's place on the line, its tiles; this CTA's share of them
   SeqSpan sp;
   int j0, nodes;                       // the block's first node and node count
   int seen;                            // slots that any of its rows can see: 0 .. seen - 1
@@ -198,6 +199,12 @@ struct KaPiece {
 __device__ __forceinline__ int ka_cap(const hg_kv8_cache& C) { return C.bt_stride * KV8_PAGE; }
 __device__ __forceinline__ int ka_tiles(const hg_kv8_cache& C, const SeqSpan& sp) {
   return (int)((min((long long)sp.start + sp.n, (long long)ka_cap(C)) + KA_TILE - 1) / KA_TILE);
+}
+
+// A unit's length on the line: its tiles and what taking it up costs, about as much as KA_TAKE tiles.
+constexpr int KA_TAKE = 1;
+__device__ __forceinline__ int ka_line(const hg_kv8_cache& C, const SeqSpan& sp) {
+  return ka_tiles(C, sp) + KA_TAKE;
 }
 
 __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre, int t, int end) {
@@ -211,15 +218,17 @@ __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre
   u.s = a;
   u.sp = kv8_span(A.R, a, true);
   u.tiles = ka_tiles(A.C, u.sp);
-  const int blocks = (u.sp.n + A.npb - 1) / A.npb, k = (t - (int)pre[a]) / u.tiles;
+  const int len = u.tiles + KA_TAKE, blocks = (u.sp.n + A.npb - 1) / A.npb, k = (t - (int)pre[a]) / len;
   u.kvh = k / blocks;
   u.blk = k - u.kvh * blocks;
-  u.u0 = (int)pre[a] + k * u.tiles;
+  u.u0 = (int)pre[a] + k * len;
   u.j0 = u.blk * A.npb;
   u.nodes = min(A.npb, u.sp.n - u.j0);
   u.seen = (int)min((long long)u.sp.start + u.j0 + u.nodes, (long long)ka_cap(A.C));
-  u.lo = t - u.u0;
-  u.hi = min(end - u.u0, u.tiles);
+  // the tiles come behind the KA_TAKE places for taking the unit up; a share of those alone is empty
+  u.lo = max(t - u.u0 - KA_TAKE, 0);
+  u.hi = min(end - u.u0 - KA_TAKE, u.tiles);
+  u.next = u.u0 + len;
   return u;
 }
 // Tiles from here on show nothing to the block's rows.
@@ -258,7 +267,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   for (int s = tid; s < n_seqs; s += S::THREADS) {
     const SeqSpan sp = kv8_span(A.R, s, true);
     if ((long long)sp.start + sp.n > ka_cap(A.C)) kv8_flag(A.R.err, HG_ERR_CONTEXT);
-    pre[s + 1] = (uint32_t)ka_tiles(A.C, sp) * A.C.n_kv_heads * ((sp.n + A.npb - 1) / A.npb);
+    pre[s + 1] = (uint32_t)ka_line(A.C, sp) * A.C.n_kv_heads * ((sp.n + A.npb - 1) / A.npb);
   }
   if (tid < R) {
     sm.node[tid] = tid / A.g;
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         }
         src = next;
       }
-      t = u.u0 + u.hi;
+      t = u.next;
     }
     for (int i = max(0, n - STAGES); i < n; i++) {
       mbar_wait(&sm.full_k[i % STAGES], (i / STAGES) & 1);
@@ -385,6 +394,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
     };
     for (int t = begin; t < end;) {
       const KaPiece u = ka_piece(A, pre, t, end);
+      if (u.hi <= u.lo) break;  // the next CTA takes the unit up
       const int last = ka_last(u);
       // ---- the block's queries as digits, and what its rows see ----
       constexpr int W = S::COMPUTE / 32;
@@ -645,7 +655,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       const float mine = warp_sums(ls);
       if (lane < RT) sm.wsum[quad][rb + lane] = mine;
       bar_group();
-      const bool from0 = u.lo == 0, to_end = u.hi == u.tiles;
+      const bool from0 = t <= u.u0 + KA_TAKE, to_end = u.next <= end;
       float* part = A.part + ((size_t)cta * 2 + (from0 ? 1 : 0)) * R * (HD + 2);
       float* out = A.out + ((size_t)(u.sp.r0 + u.j0) * A.nh + u.kvh * A.g) * HD + ti;
 #pragma unroll
@@ -665,11 +675,11 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       }
       if (from0 && !to_end && tid == 0) {
         // this CTA's share is the first: the join goes on to the CTA that holds the unit's last tile
-        const int lt = u.u0 + u.tiles - 1;
+        const int lt = u.next - 1;
         A.head[cta] = make_int4(u.sp.r0 + u.j0, u.kvh, u.nodes, (int)((((long long)lt + 1) * G - 1) / T));
       }
       bar_all();
-      t = u.u0 + u.hi;
+      t = u.next;
     }
   }
   // ---- wind-down: every MMA was waited for (bounded) by its tile; free the columns ----
@@ -721,14 +731,29 @@ void check_attn(const hg_kv8_cache* c, const hg_rows* r, int n_heads) {
   kv8_need(n_heads / c->n_kv_heads <= KV8_MAX_GROUP, "more than 32 q heads per kv head");
 }
 
-// Rows of a block: the fewest of 4, 8, 16 or 32 that hold a sequence's rows for one kv head, so that a
-// single token pays for one node and a tree reads the cache as few times as possible.
+// Rows of a block: 4, 8, 16 or 32, whichever makes a ragged batch cheapest. Time of one block's pass
+// over a tile of the cache, measured with 1 to 32 blocks of each size on 32 sequences of 900 to 7000
+// slots (12 q heads, 3 kv heads, 128 dims), in the same unit: 11.8, 15.1, 25 and 41. The sequences' row
+// counts lie between 1 and max_rows; they are taken as spread evenly around their mean.
 int block_rows(const hg_rows* r, int g) {
-  const long long want = (long long)std::min(r->max_rows, r->n_rows) * g;
-  return want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 ? 16 : 32;
+  const double hi = std::min(r->max_rows, r->n_rows), mean = std::min(hi, (double)r->n_rows / r->n_seqs);
+  const double lo = std::min(hi, std::max(1.0, 2 * mean - hi));
+  constexpr double pass[4] = {11.8, 15.1, 25.0, 41.0};
+  double least = 0.0;
+  int best = 0;
+  for (int i = 0; i < 4; i++) {
+    const int R = 4 << i, npb = R / g;
+    if (npb == 0) continue;
+    double cost = 0.0;
+    for (int k = 0; k < 8; k++) cost += std::ceil(std::round(lo + (hi - lo) * (k + 0.5) / 8) / npb) * pass[i];
+    if (best == 0 || cost < least) best = R, least = cost;
+  }
+  return best;
 }
 
 size_t part_bytes(int R, int hd) { return (size_t)KA_MAX_CTAS * 2 * R * (hd + 2) * 4; }
+// scratch for any rows: the largest block has the fewest CTAs
+size_t scratch_bytes(int hd) { return part_bytes(32, hd) / KA_MAX_CTAS * 2 * KA_SMS + KA_MAX_CTAS * sizeof(int4); }
 
 template <int HD, int R>
 void launch(KaArgs& A, int device, cudaStream_t st) {
@@ -769,8 +794,7 @@ using namespace hg;
 extern "C" size_t hg_op_kv8_attn_scratch_bytes(const hg_kv8_cache* c, const hg_rows* r, int n_heads) {
   try {
     check_attn(c, r, n_heads);
-    if (r->n_seqs == 0 || r->n_rows == 0) return 256;
-    return part_bytes(block_rows(r, n_heads / c->n_kv_heads), c->head_dim) + KA_MAX_CTAS * sizeof(int4);
+    return scratch_bytes(c->head_dim);
   } catch (const std::exception&) {
     return 0;
   }
@@ -792,12 +816,12 @@ extern "C" int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_hea
     const int R = block_rows(r, A.g);
     A.npb = R / A.g;
     // tiles are numbered with 32 bits: the most that the arguments allow
-    const double tiles = ((double)r->n_rows / A.npb + r->n_seqs) * ((double)c->bt_stride / KA_PAGES + 1) * c->n_kv_heads;
+    const double tiles = ((double)r->n_rows / A.npb + r->n_seqs) * ((double)c->bt_stride / KA_PAGES + 1 + KA_TAKE) * c->n_kv_heads;
     kv8_need(tiles < 2147483647.0, "rows x table entries x kv heads out of range for one call");
     A.q = q;
     A.out = out;
-    A.part = static_cast<float*>(scratch);
-    A.head = reinterpret_cast<int4*>(static_cast<char*>(scratch) + part_bytes(R, c->head_dim));
+    A.head = static_cast<int4*>(scratch);
+    A.part = reinterpret_cast<float*>(A.head + KA_MAX_CTAS);
     Kv8Device dev(c->pool);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int d = dev.device;

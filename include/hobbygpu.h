@@ -392,8 +392,8 @@ int hg_op_kv8_read(const hg_kv8_cache* c, const hg_rows* r, float* k_out, float*
  * sees: 0..start[s]-1, its ancestors' and its own (the rows are in the cache already), softmax of
  * q . k / sqrt(head_dim). q, out: [n_rows][n_heads * head_dim] f32, n_heads / n_kv_heads at most 32.
  * Slots without a page are not seen (err HG_ERR_CONTEXT); a row that sees nothing gets zeros. scratch:
- * 16-byte aligned device buffer of hg_op_kv8_attn_scratch_bytes() bytes, its content of no meaning
- * before and after the call; calls that may overlap need one each. */
+ * 16-byte aligned device buffer of hg_op_kv8_attn_scratch_bytes() bytes (the same for every batch of one
+ * head_dim), its content of no meaning before and after the call; calls that may overlap need one each. */
 size_t hg_op_kv8_attn_scratch_bytes(const hg_kv8_cache* c, const hg_rows* r, int n_heads);
 int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_heads, const float* q, float* out, void* scratch,
                    void* stream);

@@ -207,6 +207,11 @@ __device__ __forceinline__ int ka_line(const hg_kv8_cache& C, const SeqSpan& sp)
   return ka_tiles(C, sp) + KA_TAKE;
 }
 
+// Row blocks of a sequence.
+__device__ __forceinline__ int ka_blocks(const KaArgs& A, const SeqSpan& sp) {
+  return sp.n <= A.npb ? (sp.n > 0 ? 1 : 0) : (sp.n + A.npb - 1) / A.npb;
+}
+
 __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre, int t, int end) {
   KaPiece u;
   int a = 0, b = A.R.n_seqs - 1;
@@ -218,8 +223,8 @@ __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre
   u.s = a;
   u.sp = kv8_span(A.R, a, true);
   u.tiles = ka_tiles(A.C, u.sp);
-  const int len = u.tiles + KA_TAKE, blocks = (u.sp.n + A.npb - 1) / A.npb, k = (t - (int)pre[a]) / len;
-  u.kvh = k / blocks;
+  const int len = u.tiles + KA_TAKE, blocks = ka_blocks(A, u.sp), k = (int)((uint32_t)(t - (int)pre[a]) / (uint32_t)len);
+  u.kvh = blocks == 1 ? k : k / blocks;
   u.blk = k - u.kvh * blocks;
   u.u0 = (int)pre[a] + k * len;
   u.j0 = u.blk * A.npb;
@@ -263,35 +268,45 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   pdl_wait();
   pdl_trigger();
 
-  // ---- the line of tiles: first tile of each sequence ----
-  for (int s = tid; s < n_seqs; s += S::THREADS) {
+  // ---- the line of tiles: each sequence's first place (tensor memory and barriers meanwhile) ----
+  if (warp == COPY) {
+    // after pdl_wait, never before: a kernel still running may have to allocate before it can finish
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                 "r"(S::COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else if (warp == 1) {
+    if (lane < R) {
+      sm.node[lane] = lane / A.g;
+      sm.off[lane] = sm.node[lane] * A.nh + lane % A.g;
+    }
+    if (lane == 0) {
+      for (int k = 0; k < STAGES; k++) {
+        mbar_init(&sm.full_k[k], KA_PAGES);
+        mbar_init(&sm.full_v[k], KA_PAGES);
+        mbar_init(&sm.empty_k[k], 1);
+        mbar_init(&sm.empty_v[k], 1);
+      }
+      mbar_init(&sm.sbar, 1);
+      mbar_init(&sm.obar, 1);
+      sm.fail = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+  }
+  auto places = [&](int s) -> uint32_t {
     const SeqSpan sp = kv8_span(A.R, s, true);
     if ((long long)sp.start + sp.n > ka_cap(A.C)) kv8_flag(A.R.err, HG_ERR_CONTEXT);
-    pre[s + 1] = (uint32_t)ka_line(A.C, sp) * A.C.n_kv_heads * ((sp.n + A.npb - 1) / A.npb);
+    return (uint32_t)ka_line(A.C, sp) * A.C.n_kv_heads * ka_blocks(A, sp);
+  };
+  if (n_seqs > 32) {  // many sequences: every warp loads, then warp 0 adds up
+    for (int s = tid; s < n_seqs; s += S::THREADS) pre[s + 1] = places(s);
+    __syncthreads();
   }
-  if (tid < R) {
-    sm.node[tid] = tid / A.g;
-    sm.off[tid] = sm.node[tid] * A.nh + tid % A.g;
-  }
-  if (tid == 0) {
-    pre[0] = 0;
-    for (int k = 0; k < STAGES; k++) {
-      mbar_init(&sm.full_k[k], KA_PAGES);
-      mbar_init(&sm.full_v[k], KA_PAGES);
-      mbar_init(&sm.empty_k[k], 1);
-      mbar_init(&sm.empty_v[k], 1);
-    }
-    mbar_init(&sm.sbar, 1);
-    mbar_init(&sm.obar, 1);
-    sm.fail = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
   if (warp == 0) {
+    if (lane == 0) pre[0] = 0;
     uint32_t run = 0;
     for (int s0 = 0; s0 < n_seqs; s0 += 32) {
       const int s = s0 + lane;
-      uint32_t v = s < n_seqs ? pre[s + 1] : 0;
+      uint32_t v = s >= n_seqs ? 0 : n_seqs > 32 ? pre[s + 1] : places(s);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t w = __shfl_up_sync(0xffffffffu, v, o);
@@ -301,22 +316,14 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       run += __shfl_sync(0xffffffffu, v, 31);
     }
   }
-  __syncthreads();
-  const long long T = pre[n_seqs];
-  const int G = (int)min((long long)gridDim.x, T), cta = blockIdx.x;
-  if (tid == 0) A.head[cta] = make_int4(-1, 0, 0, 0);
-  if (cta >= G) return;
-  const int begin = (int)(T * cta / G), end = (int)(T * (cta + 1) / G);
-
-  if (warp == COPY) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
-                 "r"(S::COLS));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = sm.tmem;
+  const long long T = pre[n_seqs];
+  const int G = (int)min((long long)gridDim.x, T), cta = blockIdx.x;
+  if (tid == 0) A.head[cta] = make_int4(-1, 0, 0, 0);
+  const int begin = cta < G ? (int)(T * cta / G) : 0, end = cta < G ? (int)(T * (cta + 1) / G) : 0;
 
   if (warp == COPY) {
     // =================== copy warp: lanes 0..7 fetch a page of the tile each ===================
@@ -690,35 +697,81 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   if (tid == 0 && sm.fail) kv8_flag(A.R.err, HG_ERR_TIMEOUT);
 }
 
-// The partial results of a unit whose tiles lie in several CTAs, added up in tile order: one CTA per
-// first share and four rows.
+// The partial results of a unit whose tiles lie in several CTAs, added up in a fixed order: one CTA per
+// first share and `rows` rows (1 or 4). Latency is all it costs. A row of many shares is split over four
+// strands of threads, each with eight shares' loads in flight at a time, that meet in shared memory; of
+// few shares, each strand takes a row of the four.
+constexpr int KA_STRANDS = 4, KA_BATCH = 8;
 template <int HD, int R>
-__global__ void __launch_bounds__(4 * HD) k_kv8_join(const __grid_constant__ KaArgs A) {
+__global__ void __launch_bounds__(KA_STRANDS * HD) k_kv8_join(const __grid_constant__ KaArgs A, int rows) {
+  __shared__ float ms[KA_STRANDS], ls[KA_STRANDS], os[KA_STRANDS][HD];
   pdl_wait();
   pdl_trigger();
-  const int c0 = blockIdx.x, r = blockIdx.y * 4 + threadIdx.y;
+  const int c0 = blockIdx.x, i = threadIdx.x, strand = threadIdx.y;
   const int4 h = A.head[c0];
   if (h.x < 0) return;
-  const int node = r / A.g;
-  if (node >= h.z) return;
   constexpr int P = R * (HD + 2);
-  const float* first = A.part + ((size_t)c0 * 2 + 1) * P;       // the first share's
-  const float* next = A.part + (size_t)(c0 + 1) * 2 * P;        // and the following CTAs'
-  const int n = h.w - c0;
-  float mx = first[R * HD + r];
-#pragma unroll 8
-  for (int i = 0; i < n; i++) mx = fmaxf(mx, next[(size_t)i * 2 * P + R * HD + r]);
-  const float f0 = ex2(first[R * HD + r] - mx);
-  float o = first[r * HD + threadIdx.x] * f0, tot = first[R * HD + R + r] * f0;
-#pragma unroll 8
-  for (int i = 0; i < n; i++) {
-    const float* p = next + (size_t)i * 2 * P;
-    const float f = ex2(p[R * HD + r] - mx);
-    o = __fmaf_rn(p[r * HD + threadIdx.x], f, o);
-    tot = __fmaf_rn(p[R * HD + R + r], f, tot);
+  const int n = h.w - c0 + 1;  // shares: the first in CTA c0's second place, the others in the first place
+  // shares s0, s0 + step, ... of row r
+  auto add = [&](int r, int s0, int step, float& mx, float& o, float& tot) {
+    mx = KA_NONE;
+    o = tot = 0.0f;
+    for (; s0 < n; s0 += step * KA_BATCH) {
+      float m[KA_BATCH], l[KA_BATCH], v[KA_BATCH];
+#pragma unroll
+      for (int b = 0; b < KA_BATCH; b++) {
+        const int s = s0 + b * step, at = min(s, n - 1);
+        const float* p = A.part + ((size_t)(c0 + at) * 2 + (at == 0 ? 1 : 0)) * P;
+        m[b] = s < n ? p[R * HD + r] : KA_NONE;
+        l[b] = s < n ? p[R * HD + R + r] : 0.0f;
+        v[b] = s < n ? p[r * HD + i] : 0.0f;
+      }
+      float up = mx;
+#pragma unroll
+      for (int b = 0; b < KA_BATCH; b++) up = fmaxf(up, m[b]);
+      const float al = ex2(mx - up);
+      o *= al;
+      tot *= al;
+      mx = up;
+#pragma unroll
+      for (int b = 0; b < KA_BATCH; b++) {
+        const float f = ex2(m[b] - mx);
+        o = __fmaf_rn(v[b], f, o);
+        tot = __fmaf_rn(l[b], f, tot);
+      }
+    }
+  };
+  auto put = [&](int r, float o, float tot) {
+    const int node = r / A.g;
+    A.out[((size_t)(h.x + node) * A.nh + h.y * A.g + r - node * A.g) * HD + i] = tot == 0.0f ? 0.0f : __fdiv_rn(o, tot);
+  };
+  const int have = h.z * A.g;  // rows of the block
+  float mx, o, tot;
+  if (rows > 1 && n <= KA_BATCH) {
+    const int r = blockIdx.y * rows + strand;
+    if (r >= have) return;
+    add(r, 0, 1, mx, o, tot);
+    put(r, o, tot);
+    return;
   }
-  A.out[((size_t)(h.x + node) * A.nh + h.y * A.g + r - node * A.g) * HD + threadIdx.x] =
-      tot == 0.0f ? 0.0f : __fdiv_rn(o, tot);
+  for (int r = blockIdx.y * rows; r < min(have, (int)(blockIdx.y + 1) * rows); r++) {
+    add(r, strand, KA_STRANDS, mx, o, tot);
+    __syncthreads();
+    os[strand][i] = o;
+    if (i == 0) ms[strand] = mx, ls[strand] = tot;
+    __syncthreads();
+    if (strand != 0) continue;
+#pragma unroll
+    for (int k = 1; k < KA_STRANDS; k++) mx = fmaxf(mx, ms[k]);
+    o = tot = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KA_STRANDS; k++) {
+      const float f = ex2(ms[k] - mx);
+      o = __fmaf_rn(os[k][i], f, o);
+      tot = __fmaf_rn(ls[k], f, tot);
+    }
+    put(r, o, tot);
+  }
 }
 
 // ---- host ----
@@ -756,7 +809,7 @@ size_t part_bytes(int R, int hd) { return (size_t)KA_MAX_CTAS * 2 * R * (hd + 2)
 size_t scratch_bytes(int hd) { return part_bytes(32, hd) / KA_MAX_CTAS * 2 * KA_SMS + KA_MAX_CTAS * sizeof(int4); }
 
 template <int HD, int R>
-void launch(KaArgs& A, int device, cudaStream_t st) {
+void launch(KaArgs& A, int device, double places, cudaStream_t st) {
   using S = KaShape<HD, R>;
   const size_t smem = S::OFF_SMALL + sizeof(KaSmall<R>) + (A.R.n_seqs + 1) * sizeof(uint32_t);
   constexpr size_t most = S::OFF_SMALL + sizeof(KaSmall<R>) + (KV8_MAX_SEQS + 1) * sizeof(uint32_t);
@@ -770,7 +823,9 @@ void launch(KaArgs& A, int device, cudaStream_t st) {
   }
   const int per_sm = (int)std::min<size_t>(std::min(3, 512 / S::COLS), (228 * 1024) / (smem + 1024));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(KA_SMS * per_sm);
+  // one CTA per place on the line is the most that can have work
+  const int ctas = (int)std::min((double)KA_SMS * per_sm, places);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -780,10 +835,12 @@ void launch(KaArgs& A, int device, cudaStream_t st) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_attn<HD, R>, A));
-  cfg.gridDim = dim3(KA_SMS * per_sm, R / 4);
-  cfg.blockDim = dim3(HD, 4);
+  // few places: latency, a CTA per row; many: four rows each, so that most find their share's row at once
+  const int rows = ctas < KA_SMS * per_sm ? 1 : 4;
+  cfg.gridDim = dim3(ctas, (A.g * A.npb + rows - 1) / rows);
+  cfg.blockDim = dim3(HD, KA_STRANDS);
   cfg.dynamicSmemBytes = 0;
-  kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_join<HD, R>, A));
+  kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_join<HD, R>, A, rows));
 }
 
 }  // namespace
@@ -815,9 +872,10 @@ extern "C" int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_hea
     A.g = n_heads / c->n_kv_heads;
     const int R = block_rows(r, A.g);
     A.npb = R / A.g;
-    // tiles are numbered with 32 bits: the most that the arguments allow
-    const double tiles = ((double)r->n_rows / A.npb + r->n_seqs) * ((double)c->bt_stride / KA_PAGES + 1 + KA_TAKE) * c->n_kv_heads;
-    kv8_need(tiles < 2147483647.0, "rows x table entries x kv heads out of range for one call");
+    // places on the line are numbered with 32 bits; the most that the arguments allow:
+    const double blocks = std::floor((double)r->n_rows / A.npb) + r->n_seqs;  // the most that ragged rows make
+    const double places = blocks * ((c->bt_stride + KA_PAGES - 1) / KA_PAGES + KA_TAKE) * c->n_kv_heads;
+    kv8_need(places < 2147483647.0, "rows x table entries x kv heads out of range for one call");
     A.q = q;
     A.out = out;
     A.head = static_cast<int4*>(scratch);
@@ -826,15 +884,15 @@ extern "C" int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_hea
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int d = dev.device;
     if (c->head_dim == 64) {
-      if (R == 4) launch<64, 4>(A, d, st);
-      else if (R == 8) launch<64, 8>(A, d, st);
-      else if (R == 16) launch<64, 16>(A, d, st);
-      else launch<64, 32>(A, d, st);
+      if (R == 4) launch<64, 4>(A, d, places, st);
+      else if (R == 8) launch<64, 8>(A, d, places, st);
+      else if (R == 16) launch<64, 16>(A, d, places, st);
+      else launch<64, 32>(A, d, places, st);
     } else {
-      if (R == 4) launch<128, 4>(A, d, st);
-      else if (R == 8) launch<128, 8>(A, d, st);
-      else if (R == 16) launch<128, 16>(A, d, st);
-      else launch<128, 32>(A, d, st);
+      if (R == 4) launch<128, 4>(A, d, places, st);
+      else if (R == 8) launch<128, 8>(A, d, places, st);
+      else if (R == 16) launch<128, 16>(A, d, places, st);
+      else launch<128, 32>(A, d, places, st);
     }
   })
 }

@@ -4,6 +4,7 @@
 #pragma once
 #include <climits>
 #include <string>
+#include <utility>
 
 #include "hg_device.cuh"
 #include "hg_host.h"
@@ -66,6 +67,24 @@ __device__ __forceinline__ uint8_t* kv8_block(const hg_kv8_cache& C, int s, long
   return static_cast<uint8_t*>(C.pool) + (long long)id * C.page_stride + (long long)kvh * kv8_block_bytes(C.head_dim);
 }
 
+// Sums over the warp of R values per lane: lane i gets value i % R's.
+template <int R, class T>
+__device__ __forceinline__ T warp_sums(T (&v)[R]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int half = R / 2; half > 0; half /= 2) {
+#pragma unroll
+    for (int i = 0; i < half; i++) {
+      const bool up = lane & half;
+      const T give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+    }
+  }
+#pragma unroll
+  for (int x = R; x < 32; x *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], x);
+  return v[0];
+}
+
 // ---- host ----
 inline void kv8_need(bool ok, const char* what) {
   if (!ok) throw Error(HG_ERR_INVALID, what);
@@ -126,6 +145,22 @@ struct Kv8Device {
 
 inline void kv8_launched(cudaError_t e) {
   if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
+}
+
+// Launch with programmatic stream serialization: the kernels wait (pdl_wait) before they touch memory.
+template <typename... P, typename... Args>
+inline void kv8_launch_pdl(void (*kern)(P...), dim3 grid, int threads, size_t smem, void* stream, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  kv8_launched(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
 }
 
 #define KV8_API(...)                                     \

@@ -8,7 +8,10 @@
 
 namespace hg {
 
-constexpr int KV8_WARPS = 16;
+constexpr int KV8_WARPS = 16;  // most warps of an append CTA
+constexpr int KV8_HEADS = 4;   // heads that a warp takes at a time
+constexpr int KV8_STAGE_DIMS = 2048;  // most V dims (heads x head_dim) of a page that are staged
+constexpr int KV8_PITCH = KV8_PAGE + 4;  // bytes of a staged V dim: 5 words, so that neighbouring dims spread over the banks
 
 // round-half-even(y * inv) clamped to the codes: adding 1.5 * 2^52 leaves the rounded integer in the
 // low word of the sum.
@@ -32,27 +35,106 @@ __device__ __forceinline__ double warp_max_abs(double v) {
   return __hiloint2double((int)mh, (int)ml);
 }
 
-// One CTA per (page, sequence); its warps take the (row, head) pairs of the rows that the page holds.
-// A lane owns HD / 32 neighbouring dims, so loads, q rows and K codes move as whole words, and the
-// rotation's partner dim is 16 lanes away. The norm, rotation and quantisation of k run in f64: a code
-// sits at a rounding border of its row's scale, and f32 sums in another order would move codes by one.
+// A head's row as a warp holds it: lane l has dims l H .. l H + H - 1 of each half (H = HD / 64), so a
+// dim and its rotation partner are in the same lane.
 template <int HD>
-__global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(hg_kv8_cache C, hg_rows R, hg_kv8_append_args A) {
-  constexpr int E = HD / 32;
-  const int s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+struct HeadRow {
+  static constexpr int H = HD / 64;
+  __device__ static __forceinline__ void load(const float* p, float (&x)[2 * H]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      if constexpr (H == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(p + half * (HD / 2) + lane * 2);
+        x[half * 2] = v.x, x[half * 2 + 1] = v.y;
+      } else {
+        x[half] = p[half * (HD / 2) + lane];
+      }
+    }
+  }
+  __device__ static __forceinline__ void store(float* p, const float (&x)[2 * H]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      if constexpr (H == 2) *reinterpret_cast<float2*>(p + half * (HD / 2) + lane * 2) = make_float2(x[half * 2], x[half * 2 + 1]);
+      else p[half * (HD / 2) + lane] = x[half];
+    }
+  }
+  // dim of element e
+  __device__ static __forceinline__ int dim(int e) { return (e / H) * (HD / 2) + (threadIdx.x & 31) * H + e % H; }
+};
+
+// The codes of `count` heads' rows y into slot w of a page: K as 2 H bytes per lane, V as bytes 16 apart
+// or, staged, into shared memory. Lane g < count holds head g's scale and its inverse.
+template <int HD, bool V>
+__device__ __forceinline__ void kv8_put(const double (&y)[KV8_HEADS][HD / 32], int count, uint8_t* blk, int w,
+                                        uint8_t* stage) {
+  constexpr int E = HD / 32, H = HD / 64;
+  const int lane = threadIdx.x & 31;
+  double amax = 0.0, inv;
+#pragma unroll
+  for (int g = 0; g < KV8_HEADS; g++) {
+    double a = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const double m = fabs(y[g][e]);
+      a = (m > a || m != m) ? m : a;  // a NaN stays
+    }
+    a = warp_max_abs(a);
+    if ((lane & 3) == g) amax = a;
+  }
+  const float sc = kv8_scale(amax, &inv);
+  if (lane < count) *reinterpret_cast<float*>(blk + lane * kv8_block_bytes(HD) + (V ? kv8_vs_off(HD, w) : kv8_ks_off(HD, w))) = sc;
+#pragma unroll
+  for (int g = 0; g < KV8_HEADS; g++) {
+    if (g >= count) break;
+    const double s = __shfl_sync(0xffffffffu, inv, g);
+    uint8_t* b = blk + g * kv8_block_bytes(HD);
+    int q[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) q[e] = s > 0.0 ? kv8_code(y[g][e], s) : 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int i = HeadRow<HD>::dim(e);
+      if constexpr (V) {
+        if (stage) stage[(g * HD + i) * KV8_PITCH + w] = (uint8_t)q[e];
+        else b[kv8_v_off(HD, w, i)] = (uint8_t)q[e];
+      } else if constexpr (H == 1) {
+        b[kv8_k_off(HD, w, i)] = (uint8_t)q[e];
+      } else if (e % 2 == 0) {
+        *reinterpret_cast<uint16_t*>(b + kv8_k_off(HD, w, i)) = (uint16_t)((q[e] & 255) | (q[e + 1] & 255) << 8);
+      }
+    }
+  }
+}
+
+// One CTA per (page, sequence); its warps take the page's rows in groups of up to four heads, whose
+// loads are in flight together and whose sums, roots and divisions share the lanes (lane g finishes head
+// g). k runs in f64: a code sits at a rounding border of its row's scale, and f32 sums in another order
+// would move codes by one. The V codes of a full page are turned round in shared memory, so that they
+// leave as 16-byte columns; a page that the call fills in part gets its bytes one by one.
+template <int HD>
+__global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(const __grid_constant__ hg_kv8_cache C,
+                                                              const __grid_constant__ hg_rows R,
+                                                              const __grid_constant__ hg_kv8_append_args A) {
+  constexpr int E = HD / 32, H = HD / 64;
+  extern __shared__ __align__(16) uint8_t v_stage[];
   __shared__ int pos_s[KV8_PAGE];  // position of the page's row in slot w; -1: dropped or padding
+  pdl_wait();
+  pdl_trigger();
+  const int s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const SeqSpan sp = kv8_span(R, s, true);
   const long long base = ((long long)(sp.start / KV8_PAGE) + blockIdx.x) * KV8_PAGE;  // the page's first slot
   const int j0 = (int)max(0ll, base - sp.start);
   const int nr = (int)min((long long)sp.n, base + KV8_PAGE - sp.start) - j0;
   if (nr <= 0) return;
   const int w0 = (int)(sp.start + (long long)j0 - base);
-  const uint8_t* page = kv8_block(C, s, base, 0);
+  uint8_t* page = kv8_block(C, s, base, 0);
   if (threadIdx.x < nr) {
     const int j = j0 + threadIdx.x;
     long long pos = (long long)sp.start + j;
-    int up = kv8_parent(R, sp, j);
     if (R.parent) {
+      int up = kv8_parent(R, sp, j);
       if (up == -2) {
         pos = -1;
       } else {
@@ -73,84 +155,96 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(hg_kv8_cache C, h
   }
   __syncthreads();
   const int nh = A.n_heads, nkv = C.n_kv_heads, heads = nh + 2 * nkv;
-  for (int t = warp; t < nr * heads; t += KV8_WARPS) {
-    const int r = t / heads, h = t - r * heads, w = w0 + r, row = sp.r0 + j0 + r, pos = pos_s[r];
-    const float* src = A.qkv + ((size_t)row * heads + h) * HD + lane * E;
-    float x[E];
-    if (E == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(src);
-      x[0] = v.x, x[1] = v.y, x[E - 2] = v.z, x[E - 1] = v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(src);
-      x[0] = v.x, x[1] = v.y;
-    }
-    if (h < nh) {
-      if (!A.q_out) continue;
-      float* dst = A.q_out + ((size_t)row * nh + h) * HD + lane * E;
-      float y[E];
-      if (pos < 0) {
-#pragma unroll
-        for (int e = 0; e < E; e++) y[e] = 0.0f;
-      } else {
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) ss = __fmaf_rn(x[e], x[e], ss);
-        const float rs = __fdiv_rn(1.0f, __fsqrt_rn(warp_sum(ss) / HD + A.eps));
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const int i = lane * E + e, ci = i & (HD / 2 - 1);
-          const float n = x[e] * rs * A.q_norm[i], o = __shfl_xor_sync(0xffffffffu, n, 16);
-          const float c = A.rope_cos[(size_t)pos * (HD / 2) + ci], sn = A.rope_sin[(size_t)pos * (HD / 2) + ci];
-          y[e] = lane < 16 ? n * c - o * sn : n * c + o * sn;
-        }
+  bool staged = nr == KV8_PAGE && nkv * HD <= KV8_STAGE_DIMS;
+  for (int r = 0; staged && r < nr; r++) staged = pos_s[r] >= 0;
+  const int qg = A.q_out ? (nh + KV8_HEADS - 1) / KV8_HEADS : 0, kg = (nkv + KV8_HEADS - 1) / KV8_HEADS;
+  for (int t = warp; t < nr * (qg + 2 * kg); t += warps) {
+    const int group = t / nr, r = t - group * nr, w = w0 + r, pos = pos_s[r];
+    const int kind = group < qg ? 0 : group < qg + kg ? 1 : 2;  // q, k, v
+    const int h0 = (group - (kind == 0 ? 0 : kind == 1 ? qg : qg + kg)) * KV8_HEADS;
+    const int count = min(KV8_HEADS, (kind == 0 ? nh : nkv) - h0);
+    const size_t row = (size_t)sp.r0 + j0 + r;
+    const float* src = A.qkv + (row * heads + (kind == 0 ? 0 : kind == 1 ? nh : nh + nkv) + h0) * HD;
+    if (pos < 0) {
+      if (kind == 0) {
+        const float zero[E] = {};
+        for (int g = 0; g < count; g++) HeadRow<HD>::store(A.q_out + (row * nh + h0 + g) * HD, zero);
       }
-      if (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[E - 2], y[E - 1]);
-      else *reinterpret_cast<float2*>(dst) = make_float2(y[0], y[1]);
       continue;
     }
-    if (pos < 0) continue;
-    const bool is_v = h >= nh + nkv;
-    const int kvh = h - nh - (is_v ? nkv : 0);
-    uint8_t* blk = const_cast<uint8_t*>(page) + (long long)kvh * kv8_block_bytes(HD);
-    double y[E], amax = 0.0, inv;
-    if (is_v) {
+    float x[KV8_HEADS][E];
 #pragma unroll
-      for (int e = 0; e < E; e++) y[e] = (double)x[e];
-    } else {
-      double ss = 0.0;
+    for (int g = 0; g < KV8_HEADS; g++) HeadRow<HD>::load(src + (size_t)min(g, count - 1) * HD, x[g]);
+    uint8_t* blk = page + (long long)h0 * kv8_block_bytes(HD);
+    if (kind == 2) {
+      double y[KV8_HEADS][E];
 #pragma unroll
-      for (int e = 0; e < E; e++) ss = fma((double)x[e], (double)x[e], ss);
+      for (int g = 0; g < KV8_HEADS; g++)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const double rs = 1.0 / sqrt(ss / HD + (double)A.eps);
+        for (int e = 0; e < E; e++) y[g][e] = (double)x[g][e];
+      kv8_put<HD, true>(y, count, blk, w, staged ? v_stage + (size_t)h0 * HD * KV8_PITCH : nullptr);
+      continue;
+    }
+    float gain[E], c[H], sn[H];
+    HeadRow<HD>::load(kind == 0 ? A.q_norm : A.k_norm, gain);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const int i = lane * E + e, ci = i & (HD / 2 - 1);
-        const double n = (double)x[e] * rs * (double)A.k_norm[i], o = __shfl_xor_sync(0xffffffffu, n, 16);
-        const double c = (double)A.rope_cos[(size_t)pos * (HD / 2) + ci];
-        const double sn = (double)A.rope_sin[(size_t)pos * (HD / 2) + ci];
-        y[e] = lane < 16 ? n * c - o * sn : n * c + o * sn;
+    for (int e = 0; e < H; e++) {
+      c[e] = A.rope_cos[(size_t)pos * (HD / 2) + lane * H + e];
+      sn[e] = A.rope_sin[(size_t)pos * (HD / 2) + lane * H + e];
+    }
+    if (kind == 0) {
+      float ss[KV8_HEADS];
+#pragma unroll
+      for (int g = 0; g < KV8_HEADS; g++) {
+        ss[g] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) ss[g] = __fmaf_rn(x[g][e], x[g][e], ss[g]);
       }
-    }
+      const float rs = __fdiv_rn(1.0f, __fsqrt_rn(warp_sums(ss) / HD + A.eps));  // head lane % 4
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const double m = fabs(y[e]);
-      amax = (m > amax || m != m) ? m : amax;  // a NaN stays
-    }
-    const float sc = kv8_scale(warp_max_abs(amax), &inv);
-    uint32_t word = 0;
+      for (int g = 0; g < KV8_HEADS; g++) {
+        if (g >= count) break;
+        const float f = __shfl_sync(0xffffffffu, rs, g);
+        float y[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) word |= (uint32_t)(inv > 0.0 ? kv8_code(y[e], inv) & 255 : 0) << (8 * e);
-    if (is_v) {
-#pragma unroll
-      for (int e = 0; e < E; e++) blk[kv8_v_off(HD, w, lane * E + e)] = (uint8_t)(word >> (8 * e));
-      if (lane == 0) *reinterpret_cast<float*>(blk + kv8_vs_off(HD, w)) = sc;
+        for (int e = 0; e < H; e++) {
+          const float a = x[g][e] * f * gain[e], b = x[g][H + e] * f * gain[H + e];
+          y[e] = __fmaf_rn(a, c[e], -(b * sn[e]));
+          y[H + e] = __fmaf_rn(b, c[e], a * sn[e]);
+        }
+        HeadRow<HD>::store(A.q_out + (row * nh + h0 + g) * HD, y);
+      }
     } else {
-      uint8_t* d = blk + kv8_k_off(HD, w, lane * E);
-      if (E == 4) *reinterpret_cast<uint32_t*>(d) = word;
-      else *reinterpret_cast<uint16_t*>(d) = (uint16_t)word;
-      if (lane == 0) *reinterpret_cast<float*>(blk + kv8_ks_off(HD, w)) = sc;
+      double y[KV8_HEADS][E], ss[KV8_HEADS];
+#pragma unroll
+      for (int g = 0; g < KV8_HEADS; g++) {
+        ss[g] = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          y[g][e] = (double)x[g][e];
+          ss[g] = fma(y[g][e], y[g][e], ss[g]);
+        }
+      }
+      const double rs = 1.0 / sqrt(warp_sums(ss) / HD + (double)A.eps);
+#pragma unroll
+      for (int g = 0; g < KV8_HEADS; g++) {
+        const double f = __shfl_sync(0xffffffffu, rs, g);
+#pragma unroll
+        for (int e = 0; e < H; e++) {
+          const double a = y[g][e] * f * (double)gain[e], b = y[g][H + e] * f * (double)gain[H + e];
+          y[g][e] = fma(a, (double)c[e], -(b * (double)sn[e]));
+          y[g][H + e] = fma(b, (double)c[e], a * (double)sn[e]);
+        }
+      }
+      kv8_put<HD, false>(y, count, blk, w, nullptr);
     }
+  }
+  if (!staged) return;
+  __syncthreads();
+  for (int t = threadIdx.x; t < nkv * HD; t += blockDim.x) {
+    const uint32_t* v = reinterpret_cast<const uint32_t*>(v_stage + (size_t)t * KV8_PITCH);
+    *reinterpret_cast<uint4*>(page + (long long)(t / HD) * kv8_block_bytes(HD) + kv8_v_off(HD, 0, t % HD)) =
+        make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -158,8 +252,11 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(hg_kv8_cache C, h
 // V: a thread holds one dim's 16 slots (one 16-byte load) and writes a float to each row; neighbouring
 // threads hold neighbouring dims, so both write whole lines.
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv8_read(hg_kv8_cache C, hg_rows R, float* __restrict__ ko,
+__global__ void __launch_bounds__(256) k_kv8_read(const __grid_constant__ hg_kv8_cache C,
+                                                  const __grid_constant__ hg_rows R, float* __restrict__ ko,
                                                   float* __restrict__ vo) {
+  pdl_wait();
+  pdl_trigger();
   const int s = blockIdx.y, tid = threadIdx.x, nkv = C.n_kv_heads;
   const SeqSpan sp = kv8_span(R, s, true);
   const long long base = ((long long)(sp.start / KV8_PAGE) + blockIdx.x) * KV8_PAGE;
@@ -226,10 +323,12 @@ extern "C" int hg_op_kv8_append(const hg_kv8_cache* c, const hg_rows* r, const h
     Kv8Device dev(c->pool);
     const int rows = min(r->max_rows, r->n_rows);
     const dim3 grid((rows + KV8_PAGE - 2) / KV8_PAGE + 1, r->n_seqs);
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (c->head_dim == 64) k_kv8_append<64><<<grid, 32 * KV8_WARPS, 0, st>>>(*c, *r, *a);
-    else k_kv8_append<128><<<grid, 32 * KV8_WARPS, 0, st>>>(*c, *r, *a);
-    kv8_launched(cudaGetLastError());
+    // a warp per group of heads of the rows that a page can get
+    const int groups = (a->n_heads + KV8_HEADS - 1) / KV8_HEADS + 2 * ((c->n_kv_heads + KV8_HEADS - 1) / KV8_HEADS);
+    const int warps = min((long long)KV8_WARPS, (long long)min(rows, KV8_PAGE) * groups);
+    const int dims = c->n_kv_heads * c->head_dim;
+    const size_t smem = rows >= KV8_PAGE && dims <= KV8_STAGE_DIMS ? (size_t)dims * KV8_PITCH : 0;
+    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>, grid, 32 * warps, smem, stream, *c, *r, *a);
   })
 }
 
@@ -243,9 +342,6 @@ extern "C" int hg_op_kv8_read(const hg_kv8_cache* c, const hg_rows* r, float* k_
     Kv8Device dev(c->pool);
     const int rows = min(r->max_rows, r->n_rows);
     const dim3 grid((rows + KV8_PAGE - 2) / KV8_PAGE + 1, r->n_seqs);
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (c->head_dim == 64) k_kv8_read<64><<<grid, 256, 0, st>>>(*c, *r, k_out, v_out);
-    else k_kv8_read<128><<<grid, 256, 0, st>>>(*c, *r, k_out, v_out);
-    kv8_launched(cudaGetLastError());
+    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_read<64> : k_kv8_read<128>, grid, 256, 0, stream, *c, *r, k_out, v_out);
   })
 }

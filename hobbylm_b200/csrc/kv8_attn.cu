@@ -146,24 +146,6 @@ __device__ __forceinline__ f32x2 ka_add(const uint32_t (&d)[3][2], f32x2 f, f32x
   const f32x2 hi = pack2(__int2float_rn((int)((d[2][0] << 8) + d[1][0])), __int2float_rn((int)((d[2][1] << 8) + d[1][1])));
   return fma2(hi, f256, fma2(pack2(__int2float_rn((int)d[0][0]), __int2float_rn((int)d[0][1])), f, acc));
 }
-// Sums over the warp of R values per lane: lane i < R gets value i's.
-template <int R>
-__device__ __forceinline__ float warp_sums(float (&v)[R]) {
-  const int lane = threadIdx.x & 31;
-  int o = R / 2;
-#pragma unroll
-  for (int half = R / 2; half > 0; half /= 2, o /= 2) {
-#pragma unroll
-    for (int i = 0; i < half; i++) {
-      const bool up = lane & o;
-      const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-    }
-  }
-#pragma unroll
-  for (int x = R; x < 32; x *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], x);
-  return v[0];
-}
 // Fixed point v (|v| <= KA_FIX) as signed digits v = b0 + 256 b1 + 65536 b2, one per byte.
 __device__ __forceinline__ uint32_t to_digits(uint32_t v) { return (v + 0x808080u) ^ 0x808080u; }
 

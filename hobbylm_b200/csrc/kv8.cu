@@ -8,31 +8,49 @@
 
 namespace hg {
 
-constexpr int KV8_WARPS = 16;  // most warps of an append CTA
+constexpr int KV8_WARPS = 8;   // most warps of an append CTA: three CTAs of them fit an SM's registers
 constexpr int KV8_HEADS = 4;   // heads that a warp takes at a time
 constexpr int KV8_STAGE_DIMS = 2048;  // most V dims (heads x head_dim) of a page that are staged
 constexpr int KV8_PITCH = KV8_PAGE + 4;  // bytes of a staged V dim: 5 words, so that neighbouring dims spread over the banks
 
-// round-half-even(y * inv) clamped to the codes: adding 1.5 * 2^52 leaves the rounded integer in the
-// low word of the sum.
-__device__ __forceinline__ int kv8_code(double y, double inv) {
-  const int q = __double2loint(__dadd_rn(__dmul_rn(y, inv), 6755399441055744.0));
-  return min(max(q, -127), 127);
-}
+// round-half-even(v): adding 1.5 * 2^52 leaves the rounded integer in the low word of the sum.
+__device__ __forceinline__ int kv8_round(double v) { return __double2loint(__dadd_rn(v, 6755399441055744.0)); }
 
-// Scale of a row whose greatest magnitude is amax (any NaN or infinity: NaN), and 1 / scale.
+// Scale of a row whose greatest magnitude is amax (any NaN or infinity: NaN), and 1 / scale. The
+// quotient by 127 is amax * (1 / 127) and one correction.
 __device__ __forceinline__ float kv8_scale(double amax, double* inv) {
-  const float sc = amax <= 3.402823466385288598e38 ? (float)(amax / 127.0) : __int_as_float(0x7fffffff);
-  *inv = sc > 0.0f ? 1.0 / (double)sc : 0.0;  // a zero or NaN scale: codes 0
+  const double r = 1.0 / 127.0, q = __dmul_rn(amax, r);
+  const float sc = amax <= 3.402823466385288598e38 ? (float)fma(fma(-127.0, q, amax), r, q) : __int_as_float(0x7fffffff);
+  *inv = sc > 0.0f ? __drcp_rn((double)sc) : 0.0;  // a zero or NaN scale: codes 0
   return sc;
 }
 
-// Greatest of the lanes' non-negative doubles (NaN greatest of all): their bit patterns are ordered.
+// Greatest of the lanes' non-negative doubles: their bit patterns are ordered.
 __device__ __forceinline__ double warp_max_abs(double v) {
   const uint32_t hi = (uint32_t)__double2hiint(v), lo = (uint32_t)__double2loint(v);
   const uint32_t mh = __reduce_max_sync(0xffffffffu, hi);
   const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? lo : 0u);
   return __hiloint2double((int)mh, (int)ml);
+}
+// The greatest magnitude of a row (an infinity if it holds a NaN or one).
+template <int E>
+__device__ __forceinline__ double row_max(const double (&y)[E]) {
+  double a = 0.0;
+  bool fin = true;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const double m = fabs(y[e]);
+    fin = fin && m <= 1.7976931348623157e308;
+    a = m > a ? m : a;
+  }
+  return warp_max_abs(fin ? a : __hiloint2double(0x7ff00000, 0));
+}
+template <int E>
+__device__ __forceinline__ double row_max(const float (&x)[E]) {  // NaN patterns lie above the infinities
+  uint32_t a = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) a = max(a, __float_as_uint(x[e]) & 0x7fffffffu);
+  return (double)__uint_as_float(__reduce_max_sync(0xffffffffu, a));
 }
 
 // A head's row as a warp holds it: lane l has dims l H .. l H + H - 1 of each half (H = HD / 64), so a
@@ -65,44 +83,46 @@ struct HeadRow {
 };
 
 // The codes of `count` heads' rows y into slot w of a page: K as 2 H bytes per lane, V as bytes 16 apart
-// or, staged, into shared memory. Lane g < count holds head g's scale and its inverse.
-template <int HD, bool V>
-__device__ __forceinline__ void kv8_put(const double (&y)[KV8_HEADS][HD / 32], int count, uint8_t* blk, int w,
+// or, staged, into shared memory. Lane g < count works out head g's scale and its inverse.
+template <int HD, bool V, class T>
+__device__ __forceinline__ void kv8_put(const T (&y)[KV8_HEADS][HD / 32], int count, uint8_t* blk, int w,
                                         uint8_t* stage) {
   constexpr int E = HD / 32, H = HD / 64;
   const int lane = threadIdx.x & 31;
   double amax = 0.0, inv;
 #pragma unroll
   for (int g = 0; g < KV8_HEADS; g++) {
-    double a = 0.0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const double m = fabs(y[g][e]);
-      a = (m > a || m != m) ? m : a;  // a NaN stays
-    }
-    a = warp_max_abs(a);
+    const double a = row_max(y[g]);
     if ((lane & 3) == g) amax = a;
   }
   const float sc = kv8_scale(amax, &inv);
   if (lane < count) *reinterpret_cast<float*>(blk + lane * kv8_block_bytes(HD) + (V ? kv8_vs_off(HD, w) : kv8_ks_off(HD, w))) = sc;
+  // only the rounding of a subnormal scale is coarse enough to leave a quotient above 127
+  const bool tiny = __any_sync(0xffffffffu, sc < 1.17549435e-38f && sc > 0.0f);
+  const int i0 = HeadRow<HD>::dim(0);
+  uint8_t* bk = blk + (V ? kv8_v_off(HD, w, i0) : kv8_k_off(HD, w, i0));
 #pragma unroll
   for (int g = 0; g < KV8_HEADS; g++) {
     if (g >= count) break;
     const double s = __shfl_sync(0xffffffffu, inv, g);
-    uint8_t* b = blk + g * kv8_block_bytes(HD);
+    uint8_t* b = bk + g * kv8_block_bytes(HD);
     int q[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) q[e] = s > 0.0 ? kv8_code(y[g][e], s) : 0;
+    for (int e = 0; e < E; e++) q[e] = kv8_round(__dmul_rn((double)y[g][e], s));
+    if (tiny) {
+#pragma unroll
+      for (int e = 0; e < E; e++) q[e] = min(max(q[e], -127), 127);
+    }
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int i = HeadRow<HD>::dim(e);
+      const int di = (e / H) * (HD / 2) + e % H;  // from the lane's first dim
       if constexpr (V) {
-        if (stage) stage[(g * HD + i) * KV8_PITCH + w] = (uint8_t)q[e];
-        else b[kv8_v_off(HD, w, i)] = (uint8_t)q[e];
+        if (stage) stage[(g * HD + i0 + di) * KV8_PITCH + w] = (uint8_t)q[e];
+        else b[di * KV8_PAGE] = (uint8_t)q[e];
       } else if constexpr (H == 1) {
-        b[kv8_k_off(HD, w, i)] = (uint8_t)q[e];
+        b[di * 8] = (uint8_t)q[e];  // 16 dims on are 128 bytes on
       } else if (e % 2 == 0) {
-        *reinterpret_cast<uint16_t*>(b + kv8_k_off(HD, w, i)) = (uint16_t)((q[e] & 255) | (q[e + 1] & 255) << 8);
+        *reinterpret_cast<uint16_t*>(b + (e / H) * (HD / 2) * 8) = (uint16_t)((q[e] & 255) | (q[e + 1] & 255) << 8);
       }
     }
   }
@@ -114,7 +134,7 @@ __device__ __forceinline__ void kv8_put(const double (&y)[KV8_HEADS][HD / 32], i
 // would move codes by one. The V codes of a full page are turned round in shared memory, so that they
 // leave as 16-byte columns; a page that the call fills in part gets its bytes one by one.
 template <int HD>
-__global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(const __grid_constant__ hg_kv8_cache C,
+__global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_constant__ hg_kv8_cache C,
                                                               const __grid_constant__ hg_rows R,
                                                               const __grid_constant__ hg_kv8_append_args A) {
   constexpr int E = HD / 32, H = HD / 64;
@@ -177,12 +197,7 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(const __grid_cons
     for (int g = 0; g < KV8_HEADS; g++) HeadRow<HD>::load(src + (size_t)min(g, count - 1) * HD, x[g]);
     uint8_t* blk = page + (long long)h0 * kv8_block_bytes(HD);
     if (kind == 2) {
-      double y[KV8_HEADS][E];
-#pragma unroll
-      for (int g = 0; g < KV8_HEADS; g++)
-#pragma unroll
-        for (int e = 0; e < E; e++) y[g][e] = (double)x[g][e];
-      kv8_put<HD, true>(y, count, blk, w, staged ? v_stage + (size_t)h0 * HD * KV8_PITCH : nullptr);
+      kv8_put<HD, true>(x, count, blk, w, staged ? v_stage + (size_t)h0 * HD * KV8_PITCH : nullptr);
       continue;
     }
     float gain[E], c[H], sn[H];
@@ -200,7 +215,7 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(const __grid_cons
 #pragma unroll
         for (int e = 0; e < E; e++) ss[g] = __fmaf_rn(x[g][e], x[g][e], ss[g]);
       }
-      const float rs = __fdiv_rn(1.0f, __fsqrt_rn(warp_sums(ss) / HD + A.eps));  // head lane % 4
+      const float rs = rsqrtf(warp_sums(ss) * (1.0f / HD) + A.eps);  // head lane % 4; 2 ulp
 #pragma unroll
       for (int g = 0; g < KV8_HEADS; g++) {
         if (g >= count) break;
@@ -225,7 +240,7 @@ __global__ void __launch_bounds__(32 * KV8_WARPS) k_kv8_append(const __grid_cons
           ss[g] = fma(y[g][e], y[g][e], ss[g]);
         }
       }
-      const double rs = 1.0 / sqrt(warp_sums(ss) / HD + (double)A.eps);
+      const double rs = rsqrt(warp_sums(ss) * (1.0 / HD) + (double)A.eps);
 #pragma unroll
       for (int g = 0; g < KV8_HEADS; g++) {
         const double f = __shfl_sync(0xffffffffu, rs, g);

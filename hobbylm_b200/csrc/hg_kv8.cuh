@@ -3,6 +3,8 @@
 // device memory, and the host-side argument checks of the entry points.
 #pragma once
 #include <climits>
+#include <mutex>
+#include <set>
 #include <string>
 #include <utility>
 
@@ -145,6 +147,19 @@ struct Kv8Device {
 
 inline void kv8_launched(cudaError_t e) {
   if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
+}
+
+// The kernel may use `most` bytes of dynamic shared memory on the device (told to the runtime once).
+template <typename... P>
+inline void kv8_smem_limit(void (*kern)(P...), int device, size_t most) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> told;
+  const std::pair<const void*, int> key(reinterpret_cast<const void*>(kern), device);
+  std::lock_guard<std::mutex> lock(mu);
+  if (told.count(key)) return;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  told.insert(key);
 }
 
 // Launch with programmatic stream serialization: the kernels wait (pdl_wait) before they touch memory.

@@ -53,6 +53,9 @@ __device__ __forceinline__ double row_max(const float (&x)[E]) {  // NaN pattern
   return (double)__uint_as_float(__reduce_max_sync(0xffffffffu, a));
 }
 
+// the most that an append CTA takes: two tasks' rows per warp and a page's V codes
+constexpr size_t KV8_APPEND_SMEM = (size_t)KV8_WARPS * 2 * KV8_HEADS * 128 * 4 + (size_t)KV8_STAGE_DIMS * KV8_PITCH;
+
 // A head's row as a warp holds it: lane l has dims l H .. l H + H - 1 of each half (H = HD / 64), so a
 // dim and its rotation partner are in the same lane.
 template <int HD>
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
                                                               const __grid_constant__ hg_rows R,
                                                               const __grid_constant__ hg_kv8_append_args A) {
   constexpr int E = HD / 32, H = HD / 64;
-  extern __shared__ __align__(16) uint8_t v_stage[];
+  extern __shared__ __align__(16) float rows_s[];  // per warp, two tasks' rows: [warp][2][KV8_HEADS * HD]; the staged V
   __shared__ int pos_s[KV8_PAGE];  // position of the page's row in slot w; -1: dropped or padding
   pdl_wait();
   pdl_trigger();
@@ -149,6 +152,38 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
   const int nr = (int)min((long long)sp.n, base + KV8_PAGE - sp.start) - j0;
   if (nr <= 0) return;
   const int w0 = (int)(sp.start + (long long)j0 - base);
+  const int nh = A.n_heads, nkv = C.n_kv_heads, heads = nh + 2 * nkv;
+  const int qg = A.q_out ? (nh + KV8_HEADS - 1) / KV8_HEADS : 0, kg = (nkv + KV8_HEADS - 1) / KV8_HEADS;
+  const float* rows = A.qkv + ((size_t)sp.r0 + j0) * heads * HD;  // of the page: at most 16, fewer than 2^31 floats
+  float* mine = rows_s + warp * 2 * KV8_HEADS * HD;
+  // a task: row r's heads h0 .. h0 + count - 1 of q, k or v (kind 0, 1, 2)
+  struct Task {
+    int group, r, kind, h0, count;
+    const float* src;
+  };
+  auto place = [&](Task& k) {
+    while (k.r >= nr) k.r -= nr, k.group++;
+    const int first = k.group < qg ? 0 : k.group < qg + kg ? qg : qg + kg;
+    k.kind = k.group < qg ? 0 : k.group < qg + kg ? 1 : 2;
+    k.h0 = (k.group - first) * KV8_HEADS;
+    k.count = min(KV8_HEADS, (k.kind == 0 ? nh : nkv) - k.h0);
+    k.src = rows + (k.r * heads + (k.kind == 0 ? 0 : k.kind == 1 ? nh : nh + nkv) + k.h0) * HD;
+  };
+  // its rows on their way into shared memory while the task before is worked on
+  auto fetch = [&](const Task& k, float* dst) {
+    if (k.group < qg + 2 * kg) {
+      const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst + lane * 4);
+      const float* src = k.src + lane * 4;
+#pragma unroll
+      for (int i = 0; i < KV8_HEADS * HD / 128; i++)
+        if ((i * 32 + lane) * 4 < k.count * HD)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i * 512), "l"(src + i * 128) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  Task next{0, warp, 0, 0, 0, nullptr};
+  place(next);
+  fetch(next, mine);
   uint8_t* page = kv8_block(C, s, base, 0);
   if (threadIdx.x < nr) {
     const int j = j0 + threadIdx.x;
@@ -174,17 +209,16 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
     pos_s[threadIdx.x] = (int)pos;
   }
   __syncthreads();
-  const int nh = A.n_heads, nkv = C.n_kv_heads, heads = nh + 2 * nkv;
+  uint8_t* v_stage = reinterpret_cast<uint8_t*>(rows_s + warps * 2 * KV8_HEADS * HD);
   bool staged = nr == KV8_PAGE && nkv * HD <= KV8_STAGE_DIMS;
   for (int r = 0; staged && r < nr; r++) staged = pos_s[r] >= 0;
-  const int qg = A.q_out ? (nh + KV8_HEADS - 1) / KV8_HEADS : 0, kg = (nkv + KV8_HEADS - 1) / KV8_HEADS;
-  for (int t = warp; t < nr * (qg + 2 * kg); t += warps) {
-    const int group = t / nr, r = t - group * nr, w = w0 + r, pos = pos_s[r];
-    const int kind = group < qg ? 0 : group < qg + kg ? 1 : 2;  // q, k, v
-    const int h0 = (group - (kind == 0 ? 0 : kind == 1 ? qg : qg + kg)) * KV8_HEADS;
-    const int count = min(KV8_HEADS, (kind == 0 ? nh : nkv) - h0);
-    const size_t row = (size_t)sp.r0 + j0 + r;
-    const float* src = A.qkv + (row * heads + (kind == 0 ? 0 : kind == 1 ? nh : nh + nkv) + h0) * HD;
+  for (int odd = 0; next.group < qg + 2 * kg; odd ^= 1) {
+    const Task k = next;
+    next.r += warps;
+    place(next);
+    fetch(next, mine + (odd ^ 1) * KV8_HEADS * HD);
+    const int kind = k.kind, h0 = k.h0, count = k.count, w = w0 + k.r, pos = pos_s[k.r];
+    const size_t row = (size_t)sp.r0 + j0 + k.r;
     if (pos < 0) {
       if (kind == 0) {
         const float zero[E] = {};
@@ -192,20 +226,24 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
       }
       continue;
     }
+    float gain[E], c[H], sn[H];
+    if (kind != 2) {
+      HeadRow<HD>::load(kind == 0 ? A.q_norm : A.k_norm, gain);
+      const float *cp = A.rope_cos + (size_t)pos * (HD / 2) + lane * H, *np = A.rope_sin + (size_t)pos * (HD / 2) + lane * H;
+#pragma unroll
+      for (int e = 0; e < H; e++) c[e] = cp[e], sn[e] = np[e];
+    }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
     float x[KV8_HEADS][E];
 #pragma unroll
-    for (int g = 0; g < KV8_HEADS; g++) HeadRow<HD>::load(src + (size_t)min(g, count - 1) * HD, x[g]);
+    for (int g = 0; g < KV8_HEADS; g++)
+      HeadRow<HD>::load(mine + odd * KV8_HEADS * HD + min(g, count - 1) * HD, x[g]);
+    __syncwarp();  // read before the next fetch fills this half
     uint8_t* blk = page + (long long)h0 * kv8_block_bytes(HD);
     if (kind == 2) {
       kv8_put<HD, true>(x, count, blk, w, staged ? v_stage + (size_t)h0 * HD * KV8_PITCH : nullptr);
       continue;
-    }
-    float gain[E], c[H], sn[H];
-    HeadRow<HD>::load(kind == 0 ? A.q_norm : A.k_norm, gain);
-#pragma unroll
-    for (int e = 0; e < H; e++) {
-      c[e] = A.rope_cos[(size_t)pos * (HD / 2) + lane * H + e];
-      sn[e] = A.rope_sin[(size_t)pos * (HD / 2) + lane * H + e];
     }
     if (kind == 0) {
       float ss[KV8_HEADS];
@@ -254,6 +292,7 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
       kv8_put<HD, false>(y, count, blk, w, nullptr);
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (!staged) return;
   __syncthreads();
   for (int t = threadIdx.x; t < nkv * HD; t += blockDim.x) {
@@ -342,8 +381,11 @@ extern "C" int hg_op_kv8_append(const hg_kv8_cache* c, const hg_rows* r, const h
     const int groups = (a->n_heads + KV8_HEADS - 1) / KV8_HEADS + 2 * ((c->n_kv_heads + KV8_HEADS - 1) / KV8_HEADS);
     const int warps = min((long long)KV8_WARPS, (long long)min(rows, KV8_PAGE) * groups);
     const int dims = c->n_kv_heads * c->head_dim;
-    const size_t smem = rows >= KV8_PAGE && dims <= KV8_STAGE_DIMS ? (size_t)dims * KV8_PITCH : 0;
-    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>, grid, 32 * warps, smem, stream, *c, *r, *a);
+    const size_t smem = (size_t)warps * 2 * KV8_HEADS * c->head_dim * 4 +
+                        (rows >= KV8_PAGE && dims <= KV8_STAGE_DIMS ? (size_t)dims * KV8_PITCH : 0);
+    auto kern = c->head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>;
+    kv8_smem_limit(kern, dev.device, KV8_APPEND_SMEM);
+    kv8_launch_pdl(kern, grid, 32 * warps, smem, stream, *c, *r, *a);
   })
 }
 

@@ -24,7 +24,6 @@
 // one gives up, the CTA reports HG_ERR_TIMEOUT, waits for nothing more but its copies and MMAs
 // (bounded again), frees its tensor memory and returns.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 
 #include "hg_kv8.cuh"
@@ -795,14 +794,7 @@ void launch(KaArgs& A, int device, double places, cudaStream_t st) {
   using S = KaShape<HD, R>;
   const size_t smem = S::OFF_SMALL + sizeof(KaSmall<R>) + (A.R.n_seqs + 1) * sizeof(uint32_t);
   constexpr size_t most = S::OFF_SMALL + sizeof(KaSmall<R>) + (KV8_MAX_SEQS + 1) * sizeof(uint32_t);
-  static std::atomic<uint64_t> ready{0};  // devices whose kernel has its shared-memory limit set
-  const uint64_t bit = 1ull << (device & 63);
-  if (device > 63 || !(ready.load() & bit)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_kv8_attn<HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
-    if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-    if (device <= 63) ready.fetch_or(bit);
-  }
+  kv8_smem_limit(k_kv8_attn<HD, R>, device, most);
   const int per_sm = (int)std::min<size_t>(std::min(3, 512 / S::COLS), (228 * 1024) / (smem + 1024));
   cudaLaunchConfig_t cfg{};
   // one CTA per place on the line is the most that can have work

@@ -23,13 +23,14 @@ namespace hg {
 namespace cg = cooperative_groups;
 
 constexpr int LR_THREADS = 256;
-constexpr int LR_CHUNK = 25600;            // ids of a chunk with 16-bit words (half as many with 32)
-constexpr size_t LR_SMEM = LR_CHUNK * 2 + 32;
+constexpr int LR_CHUNK = 25216;            // most ids of a chunk with 16-bit words (half as many with 32): half a
+                                           // row of 50304, four CTAs of which fit an SM
+constexpr int LR_SPARE = 32;               // bytes behind the words that whole lines reach into
 constexpr int LR_LONG = 1 << 13;           // occurrences that a 16-bit word's 13 bits do not hold
 constexpr int LR_PATH = 256;               // drafted tokens of a path in hand at a time
 constexpr int LR_AHEAD = 4;                // 16-byte lines of a thread in flight
 constexpr int LR_BATCH = 4;                // list entries of a thread in flight
-constexpr int LR_WORK = 512;               // entries of a work list; what does not fit is done where it is claimed
+constexpr int LR_WORK = 256;               // entries of a work list; what does not fit is done where it is claimed
 constexpr int LR_OFTEN = 8;                // occurrences from which an id is for the warp that does those
 
 // The sequence that a row belongs to (-1: none): every thread of the block gets it.
@@ -127,10 +128,10 @@ struct RulesShared {
   unsigned long long red[LR_THREADS / 32], best[8];
 };
 
-// One CTA's ids lo .. hi - 1 of a row; returns the thread's greatest as an argmax key.
+// One CTA's ids lo .. hi - 1 of a row, with room for the 16-bit words of `room` ids (even); returns the thread's greatest as an argmax key.
 template <bool VEC, bool WIDE>
 __device__ __forceinline__ unsigned long long rules_run(const hg_rows& R, const RulesRow& A, RulesShared& sh,
-                                                        uint32_t* words_s, int lo, int hi) {
+                                                        uint32_t* words_s, int room, int lo, int hi) {
   using Words = RuleWords<WIDE>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float* in = A.in;
@@ -200,10 +201,10 @@ __device__ __forceinline__ unsigned long long rules_run(const hg_rows& R, const 
     }
   };
 
-  constexpr int CHUNK = WIDE ? LR_CHUNK / 2 : LR_CHUNK;
-  for (int c0 = lo; c0 < hi; c0 += CHUNK) {
+  const int chunk = WIDE ? room / 2 : room;
+  for (int c0 = lo; c0 < hi; c0 += chunk) {
     // id i's word is number i - c1, so that a line of the row has its words together; c1 <= c0
-    const int n = min(CHUNK, hi - c0), c1 = c0 - ((c0 + lines) & 3);
+    const int n = min(chunk, hi - c0), c1 = c0 - ((c0 + lines) & 3);
     // whole lines: ids ia .. ib - 1; at most three ids stand before and three behind them
     const int ia = VEC ? min(c0 + n, c1 + (c1 < c0 ? 4 : 0)) : c0 + n, ib = ia + (c0 + n - ia) / 4 * 4;
     if (VEC && tid == 0 && ib > ia)  // the run on its way to the L2 cache while the lists are gone through
@@ -337,7 +338,7 @@ __device__ __forceinline__ unsigned long long rules_run(const hg_rows& R, const 
 template <bool VEC>
 __global__ void __launch_bounds__(LR_THREADS, 4) k_logits_rules(const __grid_constant__ hg_rows R,
                                                                const __grid_constant__ hg_logits_rules_args A, int nc,
-                                                               int per) {
+                                                               int per, int room) {
   extern __shared__ __align__(16) uint32_t words_s[];
   __shared__ RulesShared sh;
   pdl_wait();
@@ -371,8 +372,8 @@ __global__ void __launch_bounds__(LR_THREADS, 4) k_logits_rules(const __grid_con
   w.token = A.token ? A.token + w.sp.r0 : nullptr;
   w.valid = A.valid > 0 ? min(A.valid, A.vocab) : A.vocab;
   const int lo = part * per, hi = min(A.vocab, lo + per);
-  unsigned long long best = (long long)w.hn + w.j + 1 < LR_LONG ? rules_run<VEC, false>(R, w, sh, words_s, lo, hi)
-                                                               : rules_run<VEC, true>(R, w, sh, words_s, lo, hi);
+  unsigned long long best = (long long)w.hn + w.j + 1 < LR_LONG ? rules_run<VEC, false>(R, w, sh, words_s, room, lo, hi)
+                                                               : rules_run<VEC, true>(R, w, sh, words_s, room, lo, hi);
   if (!A.next_ids) return;
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) sh.red[warp] = best;
@@ -421,8 +422,9 @@ extern "C" int hg_op_logits_rules(const hg_rows* r, const hg_logits_rules_args* 
     // rows move in 16-byte lines where both lie alike in them
     const bool vec = a.ld % 4 == a.ld_out % 4 && ((uintptr_t)a.logits & 15) == ((uintptr_t)a.out & 15);
     auto kern = vec ? k_logits_rules<true> : k_logits_rules<false>;
-    const size_t smem = std::min((size_t)per * 4 + 32, LR_SMEM);  // enough for words of either width
-    kv8_smem_limit(kern, dev.device, LR_SMEM);
+    const int room = std::min((per + 1) / 2 * 2, LR_CHUNK);
+    const size_t smem = (size_t)room * 2 + LR_SPARE;
+    kv8_smem_limit(kern, dev.device, LR_CHUNK * 2 + LR_SPARE);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)r->n_rows * nc);
     cfg.blockDim = dim3(LR_THREADS);
@@ -436,6 +438,6 @@ extern "C" int hg_op_logits_rules(const hg_rows* r, const hg_logits_rules_args* 
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    kv8_launched(cudaLaunchKernelEx(&cfg, kern, *r, a, nc, per));
+    kv8_launched(cudaLaunchKernelEx(&cfg, kern, *r, a, nc, per, room));
   })
 }

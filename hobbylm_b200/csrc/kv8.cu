@@ -302,53 +302,116 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
   }
 }
 
-// One CTA per (page, sequence). K: a thread turns four neighbouring codes of one slot into a float4.
-// V: a thread holds one dim's 16 slots (one 16-byte load) and writes a float to each row; neighbouring
-// threads hold neighbouring dims, so both write whole lines.
+// One CTA per `pages` neighbouring pages of a sequence for K and one for V, its work the pages' (page,
+// head) blocks. K: a thread turns four neighbouring codes of a slot into a float4. V: a thread loads one
+// dim's 16 slots; four neighbouring threads exchange their words, so that each holds four slots of four
+// dims and writes a float4 to each. Bound by the f32 rows it writes; the codes come from the L2 cache, for
+// which a CTA's pages are asked for at its start.
+constexpr int KV8_READ = 4;        // blocks of a thread in flight
+constexpr int KV8_READ_PAGES = 4;  // most pages of a CTA
+
+__device__ __forceinline__ float4 kv8_values(uint32_t codes, float sc) {
+  return make_float4((float)(int8_t)codes * sc, (float)(int8_t)(codes >> 8) * sc, (float)(int8_t)(codes >> 16) * sc,
+                     (float)(int8_t)(codes >> 24) * sc);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(const __grid_constant__ hg_kv8_cache C,
                                                   const __grid_constant__ hg_rows R, float* __restrict__ ko,
-                                                  float* __restrict__ vo) {
+                                                  float* __restrict__ vo, int pages) {
+  __shared__ const uint8_t* page_s[KV8_READ_PAGES];
   pdl_wait();
   pdl_trigger();
   const int s = blockIdx.y, tid = threadIdx.x, nkv = C.n_kv_heads;
   const SeqSpan sp = kv8_span(R, s, true);
-  const long long base = ((long long)(sp.start / KV8_PAGE) + blockIdx.x) * KV8_PAGE;
+  // the CTA's slots: base .. base + 16 pages - 1, of which its rows j0 .. j0 + nr - 1
+  const long long base = ((long long)(sp.start / KV8_PAGE) + (long long)blockIdx.x * pages) * KV8_PAGE;
   const int j0 = (int)max(0ll, base - sp.start);
-  const int nr = (int)min((long long)sp.n, base + KV8_PAGE - sp.start) - j0;
+  const int nr = (int)min((long long)sp.n, base + pages * KV8_PAGE - sp.start) - j0;
   if (nr <= 0) return;
-  const int w0 = (int)(sp.start + (long long)j0 - base);
-  const uint8_t* page = kv8_block(C, s, base, 0);
-  if (!page && tid == 0) kv8_flag(R.err, HG_ERR_CONTEXT);
-  const size_t row0 = (size_t)sp.r0 + j0, rs = (size_t)nkv * HD;
-  if (ko) {
-    for (int t = tid; t < nr * nkv * (HD / 4); t += blockDim.x) {
-      const int i = (t % (HD / 4)) * 4, kvh = (t / (HD / 4)) % nkv, r = t / (HD / 4) / nkv, w = w0 + r;
-      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (page) {
-        const uint8_t* blk = page + (long long)kvh * kv8_block_bytes(HD);
-        const char4 c = *reinterpret_cast<const char4*>(blk + kv8_k_off(HD, w, i));
-        const float sc = *reinterpret_cast<const float*>(blk + kv8_ks_off(HD, w));
-        y = make_float4(c.x * sc, c.y * sc, c.z * sc, c.w * sc);
+  const int w0 = (int)(sp.start + (long long)j0 - base), used = (w0 + nr + KV8_PAGE - 1) / KV8_PAGE;
+  if (tid < used) {
+    page_s[tid] = kv8_block(C, s, base + tid * KV8_PAGE, 0);
+    if (!page_s[tid]) kv8_flag(R.err, HG_ERR_CONTEXT);
+    else if (pages > 1 && blockIdx.z == 0)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(page_s[tid]), "r"(nkv * kv8_block_bytes(HD)) : "memory");
+  }
+  __syncthreads();
+  const size_t rs = (size_t)nkv * HD;
+  const int blocks = used * nkv;
+  const uint32_t inv = nkv == 1 ? 0u : 0xffffffffu / nkv + 1;  // q / nkv = high word of q * inv: q * nkv < 2^32
+  auto page_of = [&](int q) { return nkv == 1 ? q : (int)__umulhi(q, inv); };
+  if (ko && blockIdx.z == 0) {
+    constexpr int T = HD / 4, RT = HD / 64;  // threads of a row; rows of a block per thread, eight apart
+    const int i = tid % T * 4, wa = tid / T;
+    float* out = ko + ((size_t)sp.r0 + j0) * rs + i;
+    for (int q0 = 0; q0 < blocks; q0 += KV8_READ) {
+      uint32_t c[KV8_READ][RT];
+      float sc[KV8_READ][RT];
+#pragma unroll
+      for (int u = 0; u < KV8_READ; u++) {
+        const int q = min(q0 + u, blocks - 1), g = page_of(q);
+        const uint8_t *page = page_s[g], *blk = page + (long long)(q - g * nkv) * kv8_block_bytes(HD);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          c[u][r] = page ? *reinterpret_cast<const uint32_t*>(blk + kv8_k_off(HD, wa + 8 * r, i)) : 0u;
+          sc[u][r] = page ? *reinterpret_cast<const float*>(blk + kv8_ks_off(HD, wa + 8 * r)) : 0.0f;
+        }
       }
-      *reinterpret_cast<float4*>(ko + (row0 + r) * rs + kvh * HD + i) = y;
+#pragma unroll
+      for (int u = 0; u < KV8_READ; u++) {
+        const int q = q0 + u, g = page_of(q);
+        if (q >= blocks) break;
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          const int row = g * KV8_PAGE + wa + 8 * r - w0;  // of the CTA's rows
+          if (row >= 0 && row < nr)
+            *reinterpret_cast<float4*>(out + (size_t)row * rs + (q - g * nkv) * HD) = kv8_values(c[u][r], sc[u][r]);
+        }
+      }
     }
   }
-  if (vo) {
-    for (int t = tid; t < nkv * HD; t += blockDim.x) {
-      const int i = t % HD, kvh = t / HD;
-      alignas(16) signed char c[16] = {};
-      float sc[16] = {};
-      if (page) {
-        const uint8_t* blk = page + (long long)kvh * kv8_block_bytes(HD);
-        *reinterpret_cast<int4*>(c) = *reinterpret_cast<const int4*>(blk + kv8_v_off(HD, 0, i));
+  if (vo && blockIdx.z == gridDim.z - 1) {
+    constexpr int B = 256 / HD;  // blocks at once
+    const int i = tid % HD, a = tid & 3;
+    float* out = vo + ((size_t)sp.r0 + j0) * rs + (i & ~3);
+    for (int q0 = 0; q0 < blocks; q0 += B * KV8_READ) {  // whole warps: the exchange needs every lane
+      uint4 c[KV8_READ];
+      float4 sc[KV8_READ];
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-          *reinterpret_cast<float4*>(sc + 4 * q) = *reinterpret_cast<const float4*>(blk + kv8_vs_off(HD, 4 * q));
+      for (int u = 0; u < KV8_READ; u++) {
+        const int q = min(q0 + u * B + tid / HD, blocks - 1), g = page_of(q);
+        const uint8_t *page = page_s[g], *blk = page + (long long)(q - g * nkv) * kv8_block_bytes(HD);
+        c[u] = page ? *reinterpret_cast<const uint4*>(blk + kv8_v_off(HD, 0, i)) : make_uint4(0, 0, 0, 0);
+        sc[u] = page ? *reinterpret_cast<const float4*>(blk + kv8_vs_off(HD, 4 * a)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
 #pragma unroll
-      for (int w = 0; w < 16; w++)
-        if (w >= w0 && w < w0 + nr) vo[(row0 + w - w0) * rs + t] = c[w] * sc[w];
+      for (int u = 0; u < KV8_READ; u++) {
+        const int q = q0 + u * B + tid / HD, g = page_of(q);
+        // word b (slots 4 b .. 4 b + 3) of thread a to word a of thread b
+        uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+#pragma unroll
+        for (int step = 1; step <= 2; step *= 2) {
+#pragma unroll
+          for (int p = 0; p < 2; p++) {
+            const int lo = step == 1 ? 2 * p : p, hi = lo + step;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, a & step ? w[lo] : w[hi], step);
+            if (a & step) w[lo] = got;
+            else w[hi] = got;
+          }
+        }
+        const float s4[4] = {sc[u].x, sc[u].y, sc[u].z, sc[u].w};
+        const int row0 = g * KV8_PAGE + 4 * a - w0;
+        float* dst = out + (long long)row0 * (long long)rs + (q - g * nkv) * HD;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          // slot e's byte of the four dims
+          const uint32_t lo = __byte_perm(w[0], w[1], e | (4 + e) << 4), hi = __byte_perm(w[2], w[3], e | (4 + e) << 4);
+          if (q < blocks && row0 + e >= 0 && row0 + e < nr)
+            *reinterpret_cast<float4*>(dst) = kv8_values(__byte_perm(lo, hi, 0x5410), s4[e]);
+          dst += rs;
+        }
+      }
     }
   }
 }
@@ -398,7 +461,10 @@ extern "C" int hg_op_kv8_read(const hg_kv8_cache* c, const hg_rows* r, float* k_
     if (r->n_seqs == 0 || r->n_rows == 0) return HG_OK;
     Kv8Device dev(c->pool);
     const int rows = min(r->max_rows, r->n_rows);
-    const dim3 grid((rows + KV8_PAGE - 2) / KV8_PAGE + 1, r->n_seqs);
-    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_read<64> : k_kv8_read<128>, grid, 256, 0, stream, *c, *r, k_out, v_out);
+    const int most = (rows + KV8_PAGE - 2) / KV8_PAGE + 1;  // pages that a sequence's rows can touch
+    // four pages a CTA once that leaves every SM several, else one
+    const int pages = (long long)most * r->n_seqs >= 148 * 4 * KV8_READ_PAGES ? KV8_READ_PAGES : 1;
+    const dim3 grid((most + pages - 1) / pages, r->n_seqs, k_out && v_out ? 2 : 1);
+    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_read<64> : k_kv8_read<128>, grid, 256, 0, stream, *c, *r, k_out, v_out, pages);
   })
 }

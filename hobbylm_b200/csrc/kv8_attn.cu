@@ -558,30 +558,6 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         c_run = fmaxf(fmaxf(c_run, fmaxf(sm.wsv[grp][0], sm.wsv[grp][1])), fmaxf(sm.wsv[grp][2], sm.wsv[grp][3]));
         const float pf = c_run > 0.0f ? __fdiv_rn(vfin, c_run) * KA_FIX : 0.0f;
         const int now = n & 1;
-        float m[RT];
-        bool grew = false;
-#pragma unroll
-        for (int r = 0; r < RT; r += 4) {
-          const float4 a = *reinterpret_cast<const float4*>(&sm.wmax[0][rb + r]), b = *reinterpret_cast<const float4*>(&sm.wmax[1][rb + r]);
-          const float4 c = *reinterpret_cast<const float4*>(&sm.wmax[2][rb + r]), d = *reinterpret_cast<const float4*>(&sm.wmax[3][rb + r]);
-          const float4 o = *reinterpret_cast<const float4*>(&sm.m[now ^ 1][rb + r]);
-          m[r] = fmaxf(fmaxf(fmaxf(a.x, b.x), fmaxf(c.x, d.x)), o.x);
-          m[r + 1] = fmaxf(fmaxf(fmaxf(a.y, b.y), fmaxf(c.y, d.y)), o.y);
-          m[r + 2] = fmaxf(fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z)), o.z);
-          m[r + 3] = fmaxf(fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w)), o.w);
-          if (ti == 0) *reinterpret_cast<float4*>(&sm.m[now][rb + r]) = make_float4(m[r], m[r + 1], m[r + 2], m[r + 3]);
-          grew = grew || m[r] > o.x || m[r + 1] > o.y || m[r + 2] > o.z || m[r + 3] > o.w;
-        }
-        if (grew) {  // the same for every thread of the group
-#pragma unroll
-          for (int r = 0; r < RT; r += 2) {
-            const float2 o = *reinterpret_cast<const float2*>(&sm.m[now ^ 1][rb + r]);
-            const float2 q2 = *reinterpret_cast<const float2*>(&sm.qs[rb + r]);
-            const f32x2 al = pack2(ex2((o.x - m[r]) * q2.x), ex2((o.y - m[r + 1]) * q2.y));
-            acc[r / 2] = mul2(acc[r / 2], al);
-            l[r / 2] = mul2(l[r / 2], al);
-          }
-        }
         if (__any_sync(0xffffffffu, vs != vfin)) {  // a NaN or infinite V scale poisons the rows that see the slot
           const float bad = vs != vfin ? __int_as_float(0x7fffffff) : 0.0f;
 #pragma unroll
@@ -591,23 +567,43 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             l[r / 2] = add2(l[r / 2], pack2(x[0] != -INFINITY ? bad : 0.0f, x[1] != -INFINITY ? bad : 0.0f));
           }
         }
-        const f32x2 pf2 = pack2(pf, pf), minus1 = pack2(-1.0f, -1.0f), big = pack2(8388608.0f, 8388608.0f);
+        const f32x2 pf2 = pack2(pf, pf), minus1 = pack2(-1.0f, -1.0f), big = pack2(8388608.0f + 32896.0f, 8388608.0f + 32896.0f);
 #pragma unroll
-        for (int r = 0; r < RT; r += 2) {
-          const float2 q2 = *reinterpret_cast<const float2*>(&sm.qs[rb + r]);
-          float x[2];
-          unpack2(mul2(fma2(pack2(m[r], m[r + 1]), minus1, s[r / 2]), pack2(q2.x, q2.y)), x[0], x[1]);
-          const f32x2 p = pack2(ex2(x[0]), ex2(x[1]));
-          l[r / 2] = add2(l[r / 2], p);
-          // p * pf in [0, KA_FIX], rounded into the low bits of 2^23 + v
-          unpack2(fma2(p, pf2, big), x[0], x[1]);
+        for (int r0 = 0; r0 < RT; r0 += 4) {  // four rows at a time, so that their maxima need not stay in registers
+          const float4 a = *reinterpret_cast<const float4*>(&sm.wmax[0][rb + r0]), b = *reinterpret_cast<const float4*>(&sm.wmax[1][rb + r0]);
+          const float4 c = *reinterpret_cast<const float4*>(&sm.wmax[2][rb + r0]), d = *reinterpret_cast<const float4*>(&sm.wmax[3][rb + r0]);
+          const float4 o = *reinterpret_cast<const float4*>(&sm.m[now ^ 1][rb + r0]), q4 = *reinterpret_cast<const float4*>(&sm.qs[rb + r0]);
+          const float4 m4 = make_float4(fmaxf(fmaxf(fmaxf(a.x, b.x), fmaxf(c.x, d.x)), o.x), fmaxf(fmaxf(fmaxf(a.y, b.y), fmaxf(c.y, d.y)), o.y),
+                                        fmaxf(fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z)), o.z), fmaxf(fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w)), o.w));
+          if (ti == 0) *reinterpret_cast<float4*>(&sm.m[now][rb + r0]) = m4;
+          const float m[4] = {m4.x, m4.y, m4.z, m4.w}, q[4] = {q4.x, q4.y, q4.z, q4.w};
+          if (m[0] > o.x || m[1] > o.y || m[2] > o.z || m[3] > o.w) {  // the same for every thread of the group
+            const f32x2 al[2] = {pack2(ex2((o.x - m[0]) * q[0]), ex2((o.y - m[1]) * q[1])),
+                                 pack2(ex2((o.z - m[2]) * q[2]), ex2((o.w - m[3]) * q[3]))};
 #pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const uint32_t d = to_digits(__float_as_uint(x[i]));
+            for (int i = 0; i < 2; i++) {
+              acc[r0 / 2 + i] = mul2(acc[r0 / 2 + i], al[i]);
+              l[r0 / 2 + i] = mul2(l[r0 / 2 + i], al[i]);
+            }
+          }
 #pragma unroll
-            for (int b = 0; b < 3; b++) {
-              const int row = ((b * R) & 7) + r + i;  // rb is a multiple of 8
-              bp_mine[b][((row >> 3) * 128 + (row & 7) * 16) - ((b * R) & 7) * 16] = (unsigned char)(d >> (8 * b));
+          for (int r = r0; r < r0 + 4; r += 2) {
+            float x[2];
+            unpack2(mul2(fma2(pack2(m[r - r0], m[r - r0 + 1]), minus1, s[r / 2]), pack2(q[r - r0], q[r - r0 + 1])), x[0], x[1]);
+            const f32x2 p = pack2(ex2(x[0]), ex2(x[1]));
+            l[r / 2] = add2(l[r / 2], p);
+            // p * pf in [0, KA_FIX], rounded into the low bits of 2^23 + 0x8080 + v: the lower digits' bytes
+            // are 128 up, which the exclusive or takes back
+            unpack2(fma2(p, pf2, big), x[0], x[1]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const uint32_t d = __float_as_uint(x[i]) ^ 0x8080u;
+#pragma unroll
+              for (int b = 0; b < 3; b++) {
+                const int row = ((b * R) & 7) + r + i;  // rb is a multiple of 8
+                // (byte 2's highest bit is the exponent's lowest, which is 0)
+                bp_mine[b][((row >> 3) * 128 + (row & 7) * 16) - ((b * R) & 7) * 16] = (unsigned char)(d >> (8 * b));
+              }
             }
           }
         }

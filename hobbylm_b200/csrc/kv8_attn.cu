@@ -761,14 +761,15 @@ void check_attn(const hg_kv8_cache* c, const hg_rows* r, int n_heads) {
   kv8_need(n_heads / c->n_kv_heads <= KV8_MAX_GROUP, "more than 32 q heads per kv head");
 }
 
-// Rows of a block: 4, 8, 16 or 32, whichever makes a ragged batch cheapest. Time of one block's pass
-// over a tile of the cache, measured with 1 to 32 blocks of each size on 32 sequences of 900 to 7000
-// slots (12 q heads, 3 kv heads, 128 dims), in the same unit: 11.8, 15.1, 25 and 41. The sequences' row
-// counts lie between 1 and max_rows; they are taken as spread evenly around their mean.
+// Rows of a block: 4, 8, 16 or 32, whichever makes a ragged batch cheapest. A block's cost, the mean of
+// the call's time per block at 64 and at 256 rows a kv head (32 sequences of 900 to 7000 slots, 12 q
+// heads, 3 kv heads, 128 dims; us): 11.2, 14.9, 25.6 and 40.4. The whole calls took 723, 466, 391 and 293
+// us at 256 rows, 29.9, 32.1, 36.5 and 53.8 us with the one block that the size just fills. The
+// sequences' row counts lie between 1 and max_rows; they are taken as spread evenly around their mean.
 int block_rows(const hg_rows* r, int g) {
   const double hi = std::min(r->max_rows, r->n_rows), mean = std::min(hi, (double)r->n_rows / r->n_seqs);
   const double lo = std::min(hi, std::max(1.0, 2 * mean - hi));
-  constexpr double pass[4] = {11.8, 15.1, 25.0, 41.0};
+  constexpr double pass[4] = {11.2, 14.9, 25.6, 40.4};
   double least = 0.0;
   int best = 0;
   for (int i = 0; i < 4; i++) {

@@ -9,8 +9,8 @@
 //
 // A row is one cluster of 1, 2, 4 or 8 CTAs, each with a run of its ids in chunks. Words have 16 bits,
 // and 32 where the lists are long enough for a count to need them. Occurrences are counted with integer
-// atomics, whose order does not matter. Lists are read four entries a thread at a time, while the run is
-// on its way to the L2 cache. The arithmetic per id is Engine::generate's (sampler.cpp, lib.rs:130-139):
+// atomics, whose order does not matter. Lists are read four entries a thread at a time, before the run is
+// asked for (behind it they took twice as long). The arithmetic per id is Engine::generate's (sampler.cpp, lib.rs:130-139):
 // one f32 rounding per occurrence, so a pick equals the engine's own.
 #include <cooperative_groups.h>
 
@@ -207,8 +207,6 @@ __device__ __forceinline__ unsigned long long rules_run(const hg_rows& R, const 
     const int n = min(chunk, hi - c0), c1 = c0 - ((c0 + lines) & 3);
     // whole lines: ids ia .. ib - 1; at most three ids stand before and three behind them
     const int ia = VEC ? min(c0 + n, c1 + (c1 < c0 ? 4 : 0)) : c0 + n, ib = ia + (c0 + n - ia) / 4 * 4;
-    if (VEC && tid == 0 && ib > ia)  // the run on its way to the L2 cache while the lists are gone through
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(in + ia), "r"((ib - ia) * 4) : "memory");
     auto inside = [&](int id) { return (uint32_t)id - (uint32_t)c0 < (uint32_t)n; };
     if (listed) {
       __syncthreads();
@@ -252,6 +250,8 @@ __device__ __forceinline__ unsigned long long rules_run(const hg_rows& R, const 
           }
         });
         __syncthreads();
+        if (VEC && tid == 0 && ib > ia)  // the run on its way to the L2 cache while the listed ids are worked on
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(in + ia), "r"((ib - ia) * 4) : "memory");
         const bool last = warp == LR_THREADS / 32 - 1;  // the warp for the ids that occur often
         const int2* list = last ? sh.often : sh.once;
         const int have = min(last ? sh.often_n : sh.once_n, LR_WORK);

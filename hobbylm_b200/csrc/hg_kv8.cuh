@@ -50,7 +50,8 @@ __device__ __forceinline__ SeqSpan kv8_span(const hg_rows& R, int s, bool with_s
   return p;
 }
 
-// The parent of row j of a span (-1: none, -2: row j is padding); one that is not below j is none.
+// The parent of row j of a span (-1: none, -2 and below: row j is padding, returned as -2); one that is
+// not below j is none.
 __device__ __forceinline__ int kv8_parent(const hg_rows& R, const SeqSpan& p, int j) {
   if (!R.parent) return j - 1;
   const int q = R.parent[p.r0 + j];
@@ -146,7 +147,9 @@ struct Kv8Device {
 };
 
 inline void kv8_launched(cudaError_t e) {
-  if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
+  if (e == cudaSuccess) return;
+  cudaGetLastError();  // reported here, not to the next call that asks
+  throw Error(HG_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
 }
 
 // The kernel may use `most` bytes of dynamic shared memory on the device (told to the runtime once).

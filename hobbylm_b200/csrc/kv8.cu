@@ -228,7 +228,9 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
     }
     float gain[E], c[H], sn[H];
     if (kind != 2) {
-      HeadRow<HD>::load(kind == 0 ? A.q_norm : A.k_norm, gain);
+      const float* g = kind == 0 ? A.q_norm : A.k_norm;
+#pragma unroll
+      for (int e = 0; e < E; e++) gain[e] = g[HeadRow<HD>::dim(e)];
       const float *cp = A.rope_cos + (size_t)pos * (HD / 2) + lane * H, *np = A.rope_sin + (size_t)pos * (HD / 2) + lane * H;
 #pragma unroll
       for (int e = 0; e < H; e++) c[e] = cp[e], sn[e] = np[e];

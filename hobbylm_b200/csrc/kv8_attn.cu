@@ -273,28 +273,34 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
-  auto places = [&](int s) -> uint32_t {
+  auto places = [&](int s) -> unsigned long long {
     const SeqSpan sp = kv8_span(A.R, s, true);
     if ((long long)sp.start + sp.n > ka_cap(A.C)) kv8_flag(A.R.err, HG_ERR_CONTEXT);
-    return (uint32_t)ka_line(A.C, sp) * A.C.n_kv_heads * ka_blocks(A, sp);
+    return (unsigned long long)ka_line(A.C, sp) * A.C.n_kv_heads * ka_blocks(A, sp);
   };
+  auto place32 = [](unsigned long long v) { return (uint32_t)min(v, (unsigned long long)INT_MAX); };
   if (n_seqs > 32) {  // many sequences: every warp loads, then warp 0 adds up
-    for (int s = tid; s < n_seqs; s += S::THREADS) pre[s + 1] = places(s);
+    for (int s = tid; s < n_seqs; s += S::THREADS) pre[s + 1] = place32(places(s));
     __syncthreads();
   }
   if (warp == 0) {
     if (lane == 0) pre[0] = 0;
-    uint32_t run = 0;
+    unsigned long long run = 0;
     for (int s0 = 0; s0 < n_seqs; s0 += 32) {
       const int s = s0 + lane;
-      uint32_t v = s >= n_seqs ? 0 : n_seqs > 32 ? pre[s + 1] : places(s);
+      unsigned long long v = s >= n_seqs ? 0 : n_seqs > 32 ? pre[s + 1] : places(s);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t w = __shfl_up_sync(0xffffffffu, v, o);
+        const unsigned long long w = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += w;
       }
-      if (s < n_seqs) pre[s + 1] = run + v;
+      if (s < n_seqs) pre[s + 1] = place32(run + v);
       run += __shfl_sync(0xffffffffu, v, 31);
+    }
+    // more than the host allowed for: offsets that give rows to several sequences
+    if (run >= INT_MAX) {
+      if (lane == 0) pre[n_seqs] = 0;
+      kv8_flag(A.R.err, HG_ERR_INVALID);
     }
   }
   tc_fence_before();
@@ -371,7 +377,8 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
     };
     const uint32_t bq_a = smem_u32(bq), bp_a = smem_u32(bp), ring_a = smem_u32(ka_raw);
     constexpr uint32_t IDESC = tc_idesc(KA_TILE, S::N);
-    int n = 0;  // tiles done by this CTA
+    int n = 0;            // tiles done by this CTA
+    int issued[2] = {0, 0};  // thread 0: commits on sbar and obar
     auto issue_scores = [&](int k) {  // thread 0: S = K . q digits
       const uint32_t a = ring_a + S::OFF_K + k * S::KSTAGE;
 #pragma unroll
@@ -379,6 +386,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::PITCH, S::PITCH, 128, 0),
                    IDESC, i > 0);
       tc_commit(&sm.sbar);
+      issued[0]++;
     };
     for (int t = begin; t < end;) {
       const KaPiece u = ka_piece(A, pre, t, end);
@@ -621,6 +629,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             tc_mma_acc(tm + S::COL_O, tc_desc(a + i * 32 * HD, 16 * HD, 128, 0),
                        tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC, i > 0);
           tc_commit(&sm.obar);
+          issued[1]++;
           if (tile + 1 < last) {  // the next tile's scores meanwhile
             ka_wait(&sm.full_k[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
             issue_scores((n + 1) % STAGES);
@@ -665,8 +674,12 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       bar_all();
       t = u.next;
     }
+    if (tid == 0 && sm.fail) {  // waits were cut short: the MMAs under way (bounded)
+      if (issued[0] > 0) mbar_wait(&sm.sbar, (issued[0] - 1) & 1);
+      if (issued[1] > 0) mbar_wait(&sm.obar, (issued[1] - 1) & 1);
+    }
   }
-  // ---- wind-down: every MMA was waited for (bounded) by its tile; free the columns ----
+  // ---- wind-down: every MMA was waited for; free the columns ----
   tc_fence_before();
   __syncthreads();
   if (warp == COPY)

@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(LR_THREADS, 4) k_logits_rules(const __grid_con
   w.sp = kv8_span(R, s, false);
   w.j = row - w.sp.r0;
   if (w.j < 0 || w.j >= w.sp.n) return;
-  if (kv8_parent(R, w.sp, w.j) == -2) {
+  if (R.parent && R.parent[row] <= -2) {
     if (A.next_ids && part == 0 && tid == 0) A.next_ids[row] = -1;
     return;
   }

@@ -350,8 +350,8 @@ typedef struct {
 
 /* Rows of a ragged batch: rows row_off[s]..row_off[s+1]-1 belong to sequence s, and its row j goes to
  * slot start[s] + j, behind the slots it holds already. parent[row] is the index j' < j (within the
- * sequence) of the row drafted before it, -1 for a row that follows the context, -2 for a padding row
- * (in no tree: not cached, seen by no row, a child of it sees only itself and the context). parent =
+ * sequence) of the row drafted before it, -1 for a row that follows the context, -2 (or below) for a
+ * padding row (in no tree: not cached, seen by no row, a child of it sees only itself and the context). parent =
  * NULL: every row follows the one before it. The position of a row is start[s] plus its number of
  * ancestors. Rows from row_off[n_seqs] on are left as they were. A parent that is not below its row
  * counts as -1 (err HG_ERR_INVALID); rows past max_rows of a sequence, and sequences with start < 0,
@@ -421,7 +421,8 @@ typedef struct {
   const int32_t* bias_id;
   const float* bias;
   const uint32_t* mask;          /* rows of mask_words words, bit i % 32 of word i / 32 = id i is allowed; or NULL */
-  const int32_t* mask_row;       /* [n_rows] mask row of each row, negative: none; NULL: row i has mask row i */
+  const int32_t* mask_row;       /* [n_rows] mask row of each row (they must exist), negative: none; NULL: row i
+                                  * has mask row i */
   int32_t mask_words;            /* at least vocab / 32, rounded up */
 } hg_logits_rules_args;
 int hg_op_logits_rules(const hg_rows* r, const hg_logits_rules_args* a, void* stream);

@@ -795,3 +795,187 @@ def test_graphs_and_streams(native):
         graphs[0].replay()
     st.synchronize()
     assert torch.equal(outs[0], b.attn(q)) and not torch.equal(outs[0], eager)
+
+
+# ---------------------------------------------------------------------------------------------
+# the variants and their borders
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nodes", [1, 2, 3, 4, 7, 8, 9, 16, 33])
+def test_attn_every_block_size(native, hd, nodes):
+    """Uniform trees that fill blocks of 4, 8, 16 and 32 rows exactly, or leave some of one."""
+    rng = np.random.default_rng(nodes + hd)
+    rows = [nodes] * 3
+    _check_attn(Batch(native, rng, (8, 2, hd), [0, 250, 385], rows, random_tree(rng, rows, 0.05), spare=1), rng)
+
+
+@pytest.mark.gpu
+def test_parents_that_break_the_rule(native):
+    """A parent that is not below its row counts as none, -7 as padding; both are the same to every call."""
+    import torch
+
+    rng = np.random.default_rng(31)
+    bad = [-1, 5, 1, -7, 4, 3, -2, 2]      # rows 1 and 4 point at or above themselves, row 5 at padding
+    good = [-1, -1, 1, -2, -1, -1, -2, 2]
+    outs = []
+    for parent in (bad, good):
+        rng = np.random.default_rng(32)
+        b = Batch(native, rng, (4, 1, 64), [21], [8], parent)
+        qkv = rng.standard_normal((8, 6, 64)).astype(np.float32)
+        q = b.append(qkv, [np.ones(64, np.float32)] * 2, rope_tables(64, 64))
+        out = b.attn(q)
+        torch.cuda.synchronize()
+        assert b.err_code() == (INVALID if parent is bad else 0)
+        logits = rng.standard_normal((8, 300)).astype(np.float32)
+        token = rng.integers(0, 300, 8).tolist()
+        ruled, nxt = _rules(native, logits, [8], parent, token, [[1, 2]], np.array([1.5], np.float32))
+        outs.append((q.cpu().numpy(), out.cpu().numpy(), b.pool_np(), ruled, nxt))
+    for x, y in zip(*outs):
+        assert np.array_equal(x, y)
+
+
+@pytest.mark.gpu
+def test_append_takes_gains_at_any_float(native):
+    """Gains and RoPE tables need only be aligned to a float."""
+    import torch
+
+    rng = np.random.default_rng(33)
+    for heads in ((4, 2, 128), (4, 2, 64)):
+        b = Batch(native, rng, heads, [3], [20])
+        hd = heads[2]
+        qkv = rng.standard_normal((20, 8, hd)).astype(np.float32)
+        gains = [(1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2)]
+        rope = rope_tables(hd, 64)
+        want, pool = b.append(qkv, gains, rope).cpu().numpy(), b.pool_np()
+        b.pool.zero_()
+        shifted = [torch.cat([torch.zeros(1, device="cuda"), t.reshape(-1)]) for t in (dev(gains[0]), dev(gains[1]), dev(rope[0]), dev(rope[1]))]
+        out = torch.empty((20, 4 * hd), device="cuda")
+        ptrs = [t.data_ptr() + 4 for t in shifted]
+        a = native.Kv8Append(n_heads=4, max_pos=64, eps=1e-5, qkv=ptr(b.a_t[0]), q_norm=ptrs[0], k_norm=ptrs[1],
+                             rope_cos=ptrs[2], rope_sin=ptrs[3], q_out=ptr(out))
+        native.check(native.lib().hg_op_kv8_append(C.byref(b.cache), C.byref(b.r), C.byref(a), None))
+        assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(b.pool_np(), pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,hist,ids", [(1000, 9000, 3), (1000, 3000, 1000), (60000, 20000, 2), (250003, 900, 250003), (250003, 12000, 40)])
+def test_rules_long_lists_and_chunks(native, vocab, hist, ids):
+    """Counts that 13 bits do not hold, more listed ids than a work list, rows of several chunks."""
+    rng = np.random.default_rng(hist + ids)
+    logits = (rng.standard_normal((3, vocab)) * 5).astype(np.float32)
+    hists = [rng.integers(0, ids, n).tolist() for n in (hist, 0, hist // 2)]
+    biases = [[(int(i), 0.25) for i in rng.integers(0, vocab, n)] for n in (5, 1500, 0)]
+    rep, freq, pres = (np.array(x, np.float32) for x in ([1.0005, 1.0, 0.999], [0.0, 0.5, 0.001], [0.1, 0.0, 0.0]))
+    masks = rng.random((2, vocab)) < 0.5
+    out, nxt = _rules(native, logits, [1] * 3, None, None, hists, rep, freq, pres, biases, 0, masks, [0, -1, 1])
+    want, got, _ = rules_ref(logits, offsets([1] * 3), None, None, hists, rep, freq, pres, biases, vocab,
+                             [masks[0], None, masks[1]], exact=False)
+    assert _same(out, want) and np.array_equal(nxt, got)
+
+
+@pytest.mark.gpu
+def test_rules_long_path(native):
+    """A drafted path of more tokens than are in hand at a time, as a tree and as a chain."""
+    rng = np.random.default_rng(35)
+    n, v = 601, 700
+    logits = rng.standard_normal((n, v)).astype(np.float32)
+    token = rng.integers(0, 50, n).tolist()
+    rep, zero = np.array([1.1], np.float32), np.zeros(1, np.float32)
+    chain = [j - 1 for j in range(n)]
+    outs = [_rules(native, logits, [n], parent, token, [[3]], rep) for parent in (chain, None)]
+    want, ids, _ = rules_ref(logits, offsets([n]), None, token, [[3]], rep, zero, zero, [[]], v, [None] * n, exact=False)
+    for out, nxt in outs:
+        assert _same(out, want) and np.array_equal(nxt, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [(0, 0), (1, 1), (2, 2), (3, 3), (1, 2)])
+def test_rules_any_alignment(native, shift):
+    """Rows that start anywhere in a 16-byte line, alike and not alike in logits and out."""
+    import torch
+
+    rng = np.random.default_rng(36)
+    v, n = 5003, 4
+    x = rng.standard_normal((n, v)).astype(np.float32)
+    src, dst = (torch.full((n * v + 8,), 4.0, device="cuda") for _ in range(2))
+    src[shift[0]:shift[0] + n * v] = dev(x).reshape(-1)
+    row_off, nxt = dev(offsets([1] * n)), torch.full((n,), -9, dtype=torch.int32, device="cuda")
+    a = native.LogitsRules(vocab=v, valid=v - 3, logits=ptr(src) + 4 * shift[0], out=ptr(dst) + 4 * shift[1], next_ids=ptr(nxt))
+    r = native.Rows(n_seqs=n, n_rows=n, max_rows=1, row_off=ptr(row_off))
+    native.check(native.lib().hg_op_logits_rules(C.byref(r), C.byref(a), None))
+    got = dst.cpu().numpy()
+    want = x.copy()
+    want[:, v - 3:] = -np.inf
+    assert np.array_equal(got[shift[1]:shift[1] + n * v].reshape(n, v), want)
+    assert (got[:shift[1]] == 4.0).all() and (got[shift[1] + n * v:] == 4.0).all()
+    assert nxt.cpu().numpy().tolist() == want.argmax(1).tolist()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(native):
+    """Each with its own scratch and outputs: the same bits as one after the other."""
+    import torch
+
+    rng = np.random.default_rng(37)
+    bs = [Batch(native, rng, (12, 3, 128), rng.integers(100, 3000, 40), [1] * 40),
+          Batch(native, rng, (8, 2, 64), rng.integers(1, 900, 30), [9] * 30)]
+    qs, want, streams = [], [], [torch.cuda.Stream() for _ in bs]
+    for b in bs:
+        b.fill(rng)
+        qs.append(dev(rng.standard_normal((b.n, b.nh, b.hd)).astype(np.float32)))
+        want.append(b.attn(qs[-1]).clone())
+    outs = [torch.zeros_like(w) for w in want]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for b, q, o, st in zip(bs, qs, outs, streams):
+            b.attn(q, st.cuda_stream, b.scratch, o)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
+FIRST_CAPTURE = """
+import sys
+sys.path[:0] = ["tests", "."]
+import numpy as np, torch, ctypes as C
+import test_kv8 as t
+from hobbylm_b200 import _native as N
+rng = np.random.default_rng(1)
+b = t.Batch(N, rng, (12, 3, 128), [40, 7], [2, 3])
+qkv = rng.standard_normal((5, 18, 128)).astype(np.float32)
+one, rope = np.ones(128, np.float32), t.rope_tables(128, 64)
+args = [t.dev(x) for x in (qkv, one, one, *rope)]
+q, out, ids = torch.zeros(5, 1536, device="cuda"), torch.zeros(5, 1536, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+a = N.Kv8Append(n_heads=12, max_pos=64, eps=1e-5, qkv=t.ptr(args[0]), q_norm=t.ptr(args[1]), k_norm=t.ptr(args[2]),
+                rope_cos=t.ptr(args[3]), rope_sin=t.ptr(args[4]), q_out=t.ptr(q))
+lr = N.LogitsRules(vocab=1536, logits=t.ptr(out), out=t.ptr(out), next_ids=t.ptr(ids))
+L, by = N.lib(), C.byref
+scratch = torch.empty(L.hg_op_kv8_attn_scratch_bytes(by(b.cache), by(b.r), 12), dtype=torch.uint8, device="cuda")
+g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+st.wait_stream(torch.cuda.current_stream())
+with torch.cuda.graph(g, stream=st):  # the process's first use of each kernel
+    s = st.cuda_stream
+    N.check(L.hg_op_kv8_append(by(b.cache), by(b.r), by(a), s))
+    N.check(L.hg_op_kv8_attn(by(b.cache), by(b.r), 12, t.ptr(q), t.ptr(out), t.ptr(scratch), s))
+    N.check(L.hg_op_logits_rules(by(b.r), by(lr), s))
+g.replay()
+torch.cuda.synchronize()
+got = out.clone(), ids.clone()
+b2 = b.append(qkv, (one, one), rope)
+want = b.attn(b2)
+assert torch.equal(got[0], want) and torch.equal(got[1].long(), want.argmax(1)), "replay differs"
+print("first capture ok")
+"""
+
+
+@pytest.mark.gpu
+def test_first_use_inside_a_capture():
+    """A process whose first call of each kernel is recorded into a graph."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CAPTURE], cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "first capture ok" in r.stdout, r.stdout[-500:] + r.stderr[-1500:]

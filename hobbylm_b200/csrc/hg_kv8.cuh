@@ -152,7 +152,8 @@ inline void kv8_launched(cudaError_t e) {
   throw Error(HG_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
 }
 
-// The kernel may use `most` bytes of dynamic shared memory on the device (told to the runtime once).
+// The kernel may use `most` bytes of dynamic shared memory, and clusters of up to 16 CTAs, on the device
+// (told to the runtime once).
 template <typename... P>
 inline void kv8_smem_limit(void (*kern)(P...), int device, size_t most) {
   static std::mutex mu;
@@ -160,7 +161,8 @@ inline void kv8_smem_limit(void (*kern)(P...), int device, size_t most) {
   const std::pair<const void*, int> key(reinterpret_cast<const void*>(kern), device);
   std::lock_guard<std::mutex> lock(mu);
   if (told.count(key)) return;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
   told.insert(key);
 }

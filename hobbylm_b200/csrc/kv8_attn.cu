@@ -23,6 +23,8 @@
 // scales, three bulk copies that need no rearranging (hg_kv8.cuh). Every mbarrier wait is bounded; when
 // one gives up, the CTA reports HG_ERR_TIMEOUT, waits for nothing more but its copies and MMAs
 // (bounded again), frees its tensor memory and returns.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -31,10 +33,13 @@
 
 namespace hg {
 
+namespace cg = cooperative_groups;
+
 constexpr int KA_TILE = 128;                      // slots of a tile: the MMA's M
 constexpr int KA_PAGES = KA_TILE / KV8_PAGE;      // pages of a tile
 constexpr int KA_SMS = 148;
 constexpr int KA_MAX_CTAS = 3 * KA_SMS;
+constexpr int KA_CLUSTER = 16;                    // most CTAs of a unit's cluster
 constexpr float KA_NONE = -1e30f;                 // maximum of a row that has seen nothing: finite, below any score
 constexpr float KA_FIX = 8323072.0f;              // 2^23 - 2^16: the greatest fixed-point value, three digits
 
@@ -76,12 +81,14 @@ struct KaSmall {
   uint32_t pages[4];         // per stage: which of the tile's pages are there
   uint32_t tmem;
   int fail;
+  int first_row, kvh, nodes;  // the unit of a cluster (nodes 0: none)
 };
 
 struct KaArgs {
   hg_kv8_cache C;
   hg_rows R;
   int nh, g, npb;  // q heads, q heads per kv head, nodes per row block
+  int cl;          // CTAs of a unit's cluster, or 0: units on the line
   const float* q;
   float* out;
   float* part;     // [CTA][2][R * (hd + 2)] partial results: rows of hd sums, then maxima, then sums of p
@@ -204,17 +211,24 @@ __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre
   u.s = a;
   u.sp = kv8_span(A.R, a, true);
   u.tiles = ka_tiles(A.C, u.sp);
-  const int len = u.tiles + KA_TAKE, blocks = ka_blocks(A, u.sp), k = (int)((uint32_t)(t - (int)pre[a]) / (uint32_t)len);
+  const int len = A.cl ? 1 : u.tiles + KA_TAKE, blocks = ka_blocks(A, u.sp);
+  const int k = A.cl ? t - (int)pre[a] : (int)((uint32_t)(t - (int)pre[a]) / (uint32_t)len);
   u.kvh = blocks == 1 ? k : k / blocks;
   u.blk = k - u.kvh * blocks;
   u.u0 = (int)pre[a] + k * len;
   u.j0 = u.blk * A.npb;
   u.nodes = min(A.npb, u.sp.n - u.j0);
   u.seen = (int)min((long long)u.sp.start + u.j0 + u.nodes, (long long)ka_cap(A.C));
+  u.next = u.u0 + len;
+  if (A.cl) {  // this CTA's part of the tiles that show something
+    const int tiles = (u.seen + KA_TILE - 1) / KA_TILE, rank = blockIdx.x % A.cl;
+    u.lo = tiles * rank / A.cl;
+    u.hi = tiles * (rank + 1) / A.cl;
+    return u;
+  }
   // the tiles come behind the KA_TAKE places for taking the unit up; a share of those alone is empty
   u.lo = max(t - u.u0 - KA_TAKE, 0);
   u.hi = min(end - u.u0 - KA_TAKE, u.tiles);
-  u.next = u.u0 + len;
   return u;
 }
 // Tiles from here on show nothing to the block's rows.
@@ -276,7 +290,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   auto places = [&](int s) -> unsigned long long {
     const SeqSpan sp = kv8_span(A.R, s, true);
     if ((long long)sp.start + sp.n > ka_cap(A.C)) kv8_flag(A.R.err, HG_ERR_CONTEXT);
-    return (unsigned long long)ka_line(A.C, sp) * A.C.n_kv_heads * ka_blocks(A, sp);
+    return (unsigned long long)(A.cl ? 1 : ka_line(A.C, sp)) * A.C.n_kv_heads * ka_blocks(A, sp);
   };
   auto place32 = [](unsigned long long v) { return (uint32_t)min(v, (unsigned long long)INT_MAX); };
   if (n_seqs > 32) {  // many sequences: every warp loads, then warp 0 adds up
@@ -309,8 +323,14 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   const uint32_t tm = sm.tmem;
   const long long T = pre[n_seqs];
   const int G = (int)min((long long)gridDim.x, T), cta = blockIdx.x;
-  if (tid == 0) A.head[cta] = make_int4(-1, 0, 0, 0);
-  const int begin = cta < G ? (int)(T * cta / G) : 0, end = cta < G ? (int)(T * (cta + 1) / G) : 0;
+  int begin = 0, end = 0;  // places on the line; of a cluster: its unit
+  if (A.cl) {
+    if (cta / A.cl < T) begin = cta / A.cl, end = begin + 1;
+    if (tid == 0) sm.nodes = 0;
+  } else {
+    if (tid == 0) A.head[cta] = make_int4(-1, 0, 0, 0);
+    if (cta < G) begin = (int)(T * cta / G), end = (int)(T * (cta + 1) / G);
+  }
 
   if (warp == COPY) {
     // =================== copy warp: lanes 0..7 fetch a page of the tile each ===================
@@ -377,8 +397,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
     };
     const uint32_t bq_a = smem_u32(bq), bp_a = smem_u32(bp), ring_a = smem_u32(ka_raw);
     constexpr uint32_t IDESC = tc_idesc(KA_TILE, S::N);
-    int n = 0;            // tiles done by this CTA
-    int issued[2] = {0, 0};  // thread 0: commits on sbar and obar
+    int n = 0;  // tiles done by this CTA
     auto issue_scores = [&](int k) {  // thread 0: S = K . q digits
       const uint32_t a = ring_a + S::OFF_K + k * S::KSTAGE;
 #pragma unroll
@@ -386,11 +405,10 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::PITCH, S::PITCH, 128, 0),
                    IDESC, i > 0);
       tc_commit(&sm.sbar);
-      issued[0]++;
     };
     for (int t = begin; t < end;) {
       const KaPiece u = ka_piece(A, pre, t, end);
-      if (u.hi <= u.lo) break;  // the next CTA takes the unit up
+      if (!A.cl && u.hi <= u.lo) break;  // the next CTA takes the unit up
       const int last = ka_last(u);
       // ---- the block's queries as digits, and what its rows see ----
       constexpr int W = S::COMPUTE / 32;
@@ -629,7 +647,6 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             tc_mma_acc(tm + S::COL_O, tc_desc(a + i * 32 * HD, 16 * HD, 128, 0),
                        tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC, i > 0);
           tc_commit(&sm.obar);
-          issued[1]++;
           if (tile + 1 < last) {  // the next tile's scores meanwhile
             ka_wait(&sm.full_k[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
             issue_scores((n + 1) % STAGES);
@@ -648,8 +665,9 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       const float mine = warp_sums(ls);
       if (lane < RT) sm.wsum[quad][rb + lane] = mine;
       bar_group();
-      const bool from0 = t <= u.u0 + KA_TAKE, to_end = u.next <= end;
-      float* part = A.part + ((size_t)cta * 2 + (from0 ? 1 : 0)) * R * (HD + 2);
+      const bool from0 = A.cl ? A.cl == 1 : t <= u.u0 + KA_TAKE, to_end = u.next <= end;
+      // where a share's sums go: of a cluster to its own shared memory (the ring is done with)
+      float* part = A.cl ? reinterpret_cast<float*>(ka_raw) : A.part + ((size_t)cta * 2 + (from0 ? 1 : 0)) * R * (HD + 2);
       float* out = A.out + ((size_t)(u.sp.r0 + u.j0) * A.nh + u.kvh * A.g) * HD + ti;
 #pragma unroll
       for (int r = 0; r < RT; r++) {
@@ -666,6 +684,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           }
         }
       }
+      if (A.cl && tid == 0) sm.first_row = u.sp.r0 + u.j0, sm.kvh = u.kvh, sm.nodes = u.nodes;
       if (from0 && !to_end && tid == 0) {
         // this CTA's share is the first: the join goes on to the CTA that holds the unit's last tile
         const int lt = u.next - 1;
@@ -674,10 +693,38 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       bar_all();
       t = u.next;
     }
-    if (tid == 0 && sm.fail) {  // waits were cut short: the MMAs under way (bounded)
-      if (issued[0] > 0) mbar_wait(&sm.sbar, (issued[0] - 1) & 1);
-      if (issued[1] > 0) mbar_wait(&sm.obar, (issued[1] - 1) & 1);
+    if (tid == 0 && sm.fail && n > 0) {  // waits were cut short: the last tile's MMAs (bounded)
+      mbar_wait(&sm.sbar, (n - 1) & 1);
+      mbar_wait(&sm.obar, (n - 1) & 1);
     }
+  }
+  if (A.cl > 1) {
+    // ---- the unit's shares, each in its CTA's shared memory: row r by CTA r % cl, in tile order ----
+    cg::this_cluster().sync();
+    const int i = tid % HD;
+    if (tid < S::COMPUTE) {
+      for (int r = blockIdx.x % A.cl + A.cl * (tid / HD); r < R; r += A.cl * (S::COMPUTE / HD)) {
+        if (sm.node[r] >= sm.nodes) continue;
+        float m[KA_CLUSTER], l[KA_CLUSTER], v[KA_CLUSTER], mx = KA_NONE, o = 0.0f, tot = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KA_CLUSTER; c++) {
+          const float* p = cg::this_cluster().map_shared_rank(reinterpret_cast<const float*>(ka_raw), min(c, A.cl - 1));
+          m[c] = c < A.cl ? p[R * HD + r] : KA_NONE;
+          l[c] = c < A.cl ? p[R * HD + R + r] : 0.0f;
+          v[c] = c < A.cl ? p[r * HD + i] : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < KA_CLUSTER; c++) mx = fmaxf(mx, m[c]);
+#pragma unroll
+        for (int c = 0; c < KA_CLUSTER; c++) {
+          const float f = ex2(m[c] - mx);
+          o = __fmaf_rn(v[c], f, o);
+          tot = __fmaf_rn(l[c], f, tot);
+        }
+        A.out[((size_t)sm.first_row * A.nh + sm.kvh * A.g + sm.off[r]) * HD + i] = tot == 0.0f ? 0.0f : __fdiv_rn(o, tot);
+      }
+    }
+    cg::this_cluster().sync();  // nobody leaves while its shared memory is read
   }
   // ---- wind-down: every MMA was waited for; free the columns ----
   tc_fence_before();
@@ -800,27 +847,39 @@ size_t part_bytes(int R, int hd) { return (size_t)KA_MAX_CTAS * 2 * R * (hd + 2)
 size_t scratch_bytes(int hd) { return part_bytes(32, hd) / KA_MAX_CTAS * 2 * KA_SMS + KA_MAX_CTAS * sizeof(int4); }
 
 template <int HD, int R>
-void launch(KaArgs& A, int device, double places, cudaStream_t st) {
+void launch(KaArgs& A, int device, double units, cudaStream_t st) {
   using S = KaShape<HD, R>;
   const size_t smem = S::OFF_SMALL + sizeof(KaSmall<R>) + (A.R.n_seqs + 1) * sizeof(uint32_t);
   constexpr size_t most = S::OFF_SMALL + sizeof(KaSmall<R>) + (KV8_MAX_SEQS + 1) * sizeof(uint32_t);
   kv8_smem_limit(k_kv8_attn<HD, R>, device, most);
   const int per_sm = (int)std::min<size_t>(std::min(3, 512 / S::COLS), (228 * 1024) / (smem + 1024));
-  cudaLaunchConfig_t cfg{};
+  const int resident = KA_SMS * per_sm;
+  // A unit per cluster, joined in it, where a table's row of pages makes so few tiles that a CTA gets
+  // three at most: one launch instead of two.
+  const int tiles = (A.C.bt_stride + KA_PAGES - 1) / KA_PAGES;
+  int cl = 1;
+  while (cl < KA_CLUSTER && tiles > 2 * cl && units * 2 * cl <= KA_SMS) cl *= 2;
+  A.cl = tiles <= 3 * cl && units * cl <= resident ? cl : 0;
   // one CTA per place on the line is the most that can have work
-  const int ctas = (int)std::min((double)KA_SMS * per_sm, places);
+  const int ctas = A.cl ? (int)units * A.cl : (int)std::min((double)resident, units * (tiles + KA_TAKE));
+  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = A.cl;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = A.cl > 1 ? 2 : 1;
   kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_attn<HD, R>, A));
+  if (A.cl) return;
   // few places: latency, a CTA per row; many: four rows each, so that most find their share's row at once
-  const int rows = ctas < KA_SMS * per_sm ? 1 : 4;
+  const int rows = ctas < resident ? 1 : 4;
+  cfg.numAttrs = 1;
   cfg.gridDim = dim3(ctas, (A.g * A.npb + rows - 1) / rows);
   cfg.blockDim = dim3(HD, KA_STRANDS);
   cfg.dynamicSmemBytes = 0;
@@ -856,9 +915,10 @@ extern "C" int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_hea
     A.g = n_heads / c->n_kv_heads;
     const int R = block_rows(r, A.g);
     A.npb = R / A.g;
-    // places on the line are numbered with 32 bits; the most that the arguments allow:
-    const double blocks = std::floor((double)r->n_rows / A.npb) + r->n_seqs;  // the most that ragged rows make
-    const double places = blocks * ((c->bt_stride + KA_PAGES - 1) / KA_PAGES + KA_TAKE) * c->n_kv_heads;
+    // the most units that ragged rows make; places on the line are numbered with 32 bits
+    const double blocks = std::min(std::floor((double)r->n_rows / A.npb) + r->n_seqs,
+                                   (double)r->n_seqs * ((std::min(r->max_rows, r->n_rows) + A.npb - 1) / A.npb));
+    const double units = blocks * c->n_kv_heads, places = units * ((c->bt_stride + KA_PAGES - 1) / KA_PAGES + KA_TAKE);
     kv8_need(places < 2147483647.0, "rows x table entries x kv heads out of range for one call");
     A.q = q;
     A.out = out;
@@ -868,15 +928,15 @@ extern "C" int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_hea
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int d = dev.device;
     if (c->head_dim == 64) {
-      if (R == 4) launch<64, 4>(A, d, places, st);
-      else if (R == 8) launch<64, 8>(A, d, places, st);
-      else if (R == 16) launch<64, 16>(A, d, places, st);
-      else launch<64, 32>(A, d, places, st);
+      if (R == 4) launch<64, 4>(A, d, units, st);
+      else if (R == 8) launch<64, 8>(A, d, units, st);
+      else if (R == 16) launch<64, 16>(A, d, units, st);
+      else launch<64, 32>(A, d, units, st);
     } else {
-      if (R == 4) launch<128, 4>(A, d, places, st);
-      else if (R == 8) launch<128, 8>(A, d, places, st);
-      else if (R == 16) launch<128, 16>(A, d, places, st);
-      else launch<128, 32>(A, d, places, st);
+      if (R == 4) launch<128, 4>(A, d, units, st);
+      else if (R == 8) launch<128, 8>(A, d, units, st);
+      else if (R == 16) launch<128, 16>(A, d, units, st);
+      else launch<128, 32>(A, d, units, st);
     }
   })
 }

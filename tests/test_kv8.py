@@ -803,11 +803,30 @@ def test_graphs_and_streams(native):
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("nodes", [1, 2, 3, 4, 7, 8, 9, 16, 33])
-def test_attn_every_block_size(native, hd, nodes):
-    """Uniform trees that fill blocks of 4, 8, 16 and 32 rows exactly, or leave some of one."""
+@pytest.mark.parametrize("extra_cols", [1, 40, 900])
+def test_attn_every_block_size(native, hd, nodes, extra_cols):
+    """Uniform trees that fill blocks of 4, 8, 16 and 32 rows exactly, or leave some of one, under tables
+    so short that a unit has its own CTA, longer (its own cluster) and long (a share of the line)."""
     rng = np.random.default_rng(nodes + hd)
     rows = [nodes] * 3
-    _check_attn(Batch(native, rng, (8, 2, hd), [0, 250, 385], rows, random_tree(rng, rows, 0.05), spare=1), rng)
+    b = Batch(native, rng, (8, 2, hd), [0, 250, 285], rows, random_tree(rng, rows, 0.05), spare=1, extra_cols=extra_cols)
+    _check_attn(b, rng)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(12, 3, 128), (8, 2, 64), (16, 8, 128)])
+def test_attn_clusters_of_every_size(native, heads):
+    """One sequence under tables from one tile to more than the largest cluster takes; the context leaves
+    some CTAs of a cluster without a tile."""
+    rng = np.random.default_rng(41)
+    for cols in (8, 16, 17, 40, 100, 200, 383, 384, 385, 500):
+        for start in (0, 3, min(cols * PAGE - 2, 700)):
+            b = Batch(native, rng, heads, [start], [2], extra_cols=1)
+            table = np.full((1, cols), 0x7fffffff, np.int32)
+            table[:, :b.table.shape[1]] = b.table[:, :cols]
+            b.table, b.t["table"] = table, dev(table)
+            b.cache.block_table, b.cache.bt_stride = ptr(b.t["table"]), cols
+            _check_attn(b, rng)
 
 
 @pytest.mark.gpu

@@ -320,14 +320,15 @@ __device__ __forceinline__ float4 kv8_values(uint32_t codes, float sc) {
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_read(const __grid_constant__ hg_kv8_cache C,
                                                   const __grid_constant__ hg_rows R, float* __restrict__ ko,
-                                                  float* __restrict__ vo, int pages) {
+                                                  float* __restrict__ vo, int pages, int kinds) {
   __shared__ const uint8_t* page_s[KV8_READ_PAGES];
   pdl_wait();
   pdl_trigger();
-  const int s = blockIdx.y, tid = threadIdx.x, nkv = C.n_kv_heads;
+  // K's and V's CTA of the same pages side by side (kinds = 2), so that they meet in the L2 cache
+  const int s = blockIdx.y, tid = threadIdx.x, nkv = C.n_kv_heads, chunk = blockIdx.x / kinds, kind = blockIdx.x % kinds;
   const SeqSpan sp = kv8_span(R, s, true);
   // the CTA's slots: base .. base + 16 pages - 1, of which its rows j0 .. j0 + nr - 1
-  const long long base = ((long long)(sp.start / KV8_PAGE) + (long long)blockIdx.x * pages) * KV8_PAGE;
+  const long long base = ((long long)(sp.start / KV8_PAGE) + (long long)chunk * pages) * KV8_PAGE;
   const int j0 = (int)max(0ll, base - sp.start);
   const int nr = (int)min((long long)sp.n, base + pages * KV8_PAGE - sp.start) - j0;
   if (nr <= 0) return;
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const __grid_constant__ hg_kv8
   if (tid < used) {
     page_s[tid] = kv8_block(C, s, base + tid * KV8_PAGE, 0);
     if (!page_s[tid]) kv8_flag(R.err, HG_ERR_CONTEXT);
-    else if (pages > 1 && blockIdx.z == 0)
+    else if (pages > 1 && kind == 0)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(page_s[tid]), "r"(nkv * kv8_block_bytes(HD)) : "memory");
   }
   __syncthreads();
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const __grid_constant__ hg_kv8
   const int blocks = used * nkv;
   const uint32_t inv = nkv == 1 ? 0u : 0xffffffffu / nkv + 1;  // q / nkv = high word of q * inv: q * nkv < 2^32
   auto page_of = [&](int q) { return nkv == 1 ? q : (int)__umulhi(q, inv); };
-  if (ko && blockIdx.z == 0) {
+  if (ko && kind == 0) {
     constexpr int T = HD / 4, RT = HD / 64;  // threads of a row; rows of a block per thread, eight apart
     const int i = tid % T * 4, wa = tid / T;
     float* out = ko + ((size_t)sp.r0 + j0) * rs + i;
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const __grid_constant__ hg_kv8
       }
     }
   }
-  if (vo && blockIdx.z == gridDim.z - 1) {
+  if (vo && kind == kinds - 1) {
     constexpr int B = 256 / HD;  // blocks at once
     const int i = tid % HD, a = tid & 3;
     float* out = vo + ((size_t)sp.r0 + j0) * rs + (i & ~3);
@@ -466,7 +467,8 @@ extern "C" int hg_op_kv8_read(const hg_kv8_cache* c, const hg_rows* r, float* k_
     const int most = (rows + KV8_PAGE - 2) / KV8_PAGE + 1;  // pages that a sequence's rows can touch
     // four pages a CTA once that leaves every SM several, else one
     const int pages = (long long)most * r->n_seqs >= 148 * 4 * KV8_READ_PAGES ? KV8_READ_PAGES : 1;
-    const dim3 grid((most + pages - 1) / pages, r->n_seqs, k_out && v_out ? 2 : 1);
-    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_read<64> : k_kv8_read<128>, grid, 256, 0, stream, *c, *r, k_out, v_out, pages);
+    const int kinds = k_out && v_out ? 2 : 1;
+    const dim3 grid((most + pages - 1) / pages * kinds, r->n_seqs);
+    kv8_launch_pdl(c->head_dim == 64 ? k_kv8_read<64> : k_kv8_read<128>, grid, 256, 0, stream, *c, *r, k_out, v_out, pages, kinds);
   })
 }

@@ -16,13 +16,25 @@
 // bytes. The running maximum, sum and output rows stay in registers from tile to tile.
 //
 // Work split: all tiles of all (sequence, kv head, row block) units lie on one line that is cut into
-// equal runs, one per resident CTA, whatever the lengths; a unit that is cut is joined by
-// k_kv8_join from at most two partial results per CTA, in tile order (no atomics).
+// equal runs, one per resident CTA, whatever the lengths; a unit that is cut is joined by k_kv8_join from
+// at most two partial results per CTA, in tile order (no atomics). Where the page tables are so short
+// that a unit has few tiles, each unit has a cluster of 1 to 16 CTAs instead, joined over distributed
+// shared memory: one launch, which is what a small call costs (one sequence of 2100 slots: 8.9 us a call
+// against 10.4).
 //
-// A copy warp keeps the stages of a ring full: per page 16 hd bytes of K, as many of V and 128 of
-// scales, three bulk copies that need no rearranging (hg_kv8.cuh). Every mbarrier wait is bounded; when
-// one gives up, the CTA reports HG_ERR_TIMEOUT, waits for nothing more but its copies and MMAs
-// (bounded again), frees its tensor memory and returns.
+// A copy warp keeps two rings full, K tiles with the scales of both and V tiles: per page 16 hd bytes of
+// K, 128 of scales and 16 hd of V, bulk copies that need no rearranging (hg_kv8.cuh). One thread issues
+// the MMAs: a tile's value product and the next tile's scores together, so that the compute warps find
+// scores ready; a tile's value sums are read back while the next tile's maxima meet. Every mbarrier wait
+// is bounded; when one gives up, the CTA reports HG_ERR_TIMEOUT, its other waits give up soon too, and it
+// waits (bounded) for its copies and last MMAs before it frees its tensor memory and returns.
+//
+// Measured: 256 sequences of 1024 to 8192 slots (12 q heads, 3 kv heads, 128 dims) 147-152 us, 5.9 TB/s
+// of cache, 0.90 of measured HBM (R = 4, three CTAs an SM: bound by HBM). 32 trees of 64 nodes over 900
+// to 7000 slots 284 us, 176 TFLOP/s of f32-exact products (R = 32, two CTAs of 288 threads an SM): bound
+// by the instructions between the products, about 50 per (slot, row): put three digits together, scale,
+// maximum, exponential, sum, three digits again, add the value sums. Issue slots are 55% busy at 17 warps
+// an SM, which 96 registers a thread allow; the tensor pipe 13%.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -736,12 +748,15 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
 
 // The partial results of a unit whose tiles lie in several CTAs, added up in a fixed order: one CTA per
 // first share and `rows` rows (1 or 4). Latency is all it costs. A row of many shares is split over four
-// strands of threads, each with eight shares' loads in flight at a time, that meet in shared memory; of
-// few shares, each strand takes a row of the four.
+// warps, each with eight shares' loads in flight at a time, that meet in shared memory; of few shares,
+// each warp takes a row of the four. A lane has HD / 32 dims of a row.
 constexpr int KA_STRANDS = 4, KA_BATCH = 8;
 template <int HD, int R>
-__global__ void __launch_bounds__(KA_STRANDS * HD) k_kv8_join(const __grid_constant__ KaArgs A, int rows) {
-  __shared__ float ms[KA_STRANDS], ls[KA_STRANDS], os[KA_STRANDS][HD];
+__global__ void __launch_bounds__(KA_STRANDS * 32) k_kv8_join(const __grid_constant__ KaArgs A, int rows) {
+  constexpr int E = HD / 32;
+  struct __align__(4 * E) Dims { float d[E]; };
+  __shared__ float ms[KA_STRANDS], ls[KA_STRANDS];
+  __shared__ Dims os[KA_STRANDS][32];
   pdl_wait();
   pdl_trigger();
   const int c0 = blockIdx.x, i = threadIdx.x, strand = threadIdx.y;
@@ -750,40 +765,47 @@ __global__ void __launch_bounds__(KA_STRANDS * HD) k_kv8_join(const __grid_const
   constexpr int P = R * (HD + 2);
   const int n = h.w - c0 + 1;  // shares: the first in CTA c0's second place, the others in the first place
   // shares s0, s0 + step, ... of row r
-  auto add = [&](int r, int s0, int step, float& mx, float& o, float& tot) {
+  auto add = [&](int r, int s0, int step, float& mx, Dims& o, float& tot) {
     mx = KA_NONE;
-    o = tot = 0.0f;
+    o = Dims{};
+    tot = 0.0f;
     for (; s0 < n; s0 += step * KA_BATCH) {
-      float m[KA_BATCH], l[KA_BATCH], v[KA_BATCH];
+      float m[KA_BATCH], l[KA_BATCH];
+      Dims v[KA_BATCH];
 #pragma unroll
       for (int b = 0; b < KA_BATCH; b++) {
         const int s = s0 + b * step, at = min(s, n - 1);
         const float* p = A.part + ((size_t)(c0 + at) * 2 + (at == 0 ? 1 : 0)) * P;
         m[b] = s < n ? p[R * HD + r] : KA_NONE;
         l[b] = s < n ? p[R * HD + R + r] : 0.0f;
-        v[b] = s < n ? p[r * HD + i] : 0.0f;
+        v[b] = s < n ? reinterpret_cast<const Dims*>(p + r * HD)[i] : Dims{};
       }
       float up = mx;
 #pragma unroll
       for (int b = 0; b < KA_BATCH; b++) up = fmaxf(up, m[b]);
       const float al = ex2(mx - up);
-      o *= al;
+#pragma unroll
+      for (int e = 0; e < E; e++) o.d[e] *= al;
       tot *= al;
       mx = up;
 #pragma unroll
       for (int b = 0; b < KA_BATCH; b++) {
         const float f = ex2(m[b] - mx);
-        o = __fmaf_rn(v[b], f, o);
+#pragma unroll
+        for (int e = 0; e < E; e++) o.d[e] = __fmaf_rn(v[b].d[e], f, o.d[e]);
         tot = __fmaf_rn(l[b], f, tot);
       }
     }
   };
-  auto put = [&](int r, float o, float tot) {
+  auto put = [&](int r, Dims o, float tot) {
     const int node = r / A.g;
-    A.out[((size_t)(h.x + node) * A.nh + h.y * A.g + r - node * A.g) * HD + i] = tot == 0.0f ? 0.0f : __fdiv_rn(o, tot);
+#pragma unroll
+    for (int e = 0; e < E; e++) o.d[e] = tot == 0.0f ? 0.0f : __fdiv_rn(o.d[e], tot);
+    reinterpret_cast<Dims*>(A.out + ((size_t)(h.x + node) * A.nh + h.y * A.g + r - node * A.g) * HD)[i] = o;
   };
   const int have = h.z * A.g;  // rows of the block
-  float mx, o, tot;
+  float mx, tot;
+  Dims o;
   if (rows > 1 && n <= KA_BATCH) {
     const int r = blockIdx.y * rows + strand;
     if (r >= have) return;
@@ -800,11 +822,13 @@ __global__ void __launch_bounds__(KA_STRANDS * HD) k_kv8_join(const __grid_const
     if (strand != 0) continue;
 #pragma unroll
     for (int k = 1; k < KA_STRANDS; k++) mx = fmaxf(mx, ms[k]);
-    o = tot = 0.0f;
+    o = Dims{};
+    tot = 0.0f;
 #pragma unroll
     for (int k = 0; k < KA_STRANDS; k++) {
       const float f = ex2(ms[k] - mx);
-      o = __fmaf_rn(os[k][i], f, o);
+#pragma unroll
+      for (int e = 0; e < E; e++) o.d[e] = __fmaf_rn(os[k][i].d[e], f, o.d[e]);
       tot = __fmaf_rn(ls[k], f, tot);
     }
     put(r, o, tot);
@@ -881,7 +905,7 @@ void launch(KaArgs& A, int device, double units, cudaStream_t st) {
   const int rows = ctas < resident ? 1 : 4;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(ctas, (A.g * A.npb + rows - 1) / rows);
-  cfg.blockDim = dim3(HD, KA_STRANDS);
+  cfg.blockDim = dim3(32, KA_STRANDS);
   cfg.dynamicSmemBytes = 0;
   kv8_launched(cudaLaunchKernelEx(&cfg, k_kv8_join<HD, R>, A, rows));
 }

@@ -10,8 +10,14 @@
 // A row is one cluster of 1, 2, 4 or 8 CTAs, each with a run of its ids in chunks. Words have 16 bits,
 // and 32 where the lists are long enough for a count to need them. Occurrences are counted with integer
 // atomics, whose order does not matter. Lists are read four entries a thread at a time, before the run is
-// asked for (behind it they took twice as long). The arithmetic per id is Engine::generate's (sampler.cpp, lib.rs:130-139):
-// one f32 rounding per occurrence, so a pick equals the engine's own.
+// asked for (behind it they took twice as long). The arithmetic per id is Engine::generate's (sampler.cpp,
+// lib.rs:130-139): one f32 rounding per occurrence, so a pick equals the engine's own.
+//
+// 256 rows of 50304 ids with histories of up to 2000 ids and up to 300 biases take 44 us, of which the
+// bytes need 16: all CTAs run at once, each through its lists (some 12 us of loads and atomics that wait
+// for one another) and then its stream (about the 16), and too few rows follow to fill the one with the
+// other. The same rows without lists take 27 us. Smaller CTAs (runs of an eighth), more of them an SM (48
+// registers) and eight list entries a thread were slower.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -135,7 +135,10 @@ struct Kv8Device {
     cudaGetDevice(&cur);
     if (cur != at.device) {
       e = cudaSetDevice(at.device);
-      if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        throw Error(HG_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+      }
       prev = cur;
     }
   }
@@ -163,7 +166,10 @@ inline void kv8_smem_limit(void (*kern)(P...), int device, size_t most) {
   if (told.count(key)) return;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) throw Error(HG_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    throw Error(HG_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  }
   told.insert(key);
 }
 

@@ -31,7 +31,7 @@
 //
 // Measured: 256 sequences of 1024 to 8192 slots (12 q heads, 3 kv heads, 128 dims) 147-152 us, 5.9 TB/s
 // of cache, 0.90 of measured HBM (R = 4, three CTAs an SM: bound by HBM). 32 trees of 64 nodes over 900
-// to 7000 slots 284 us, 176 TFLOP/s of f32-exact products (R = 32, two CTAs of 288 threads an SM): bound
+// to 7000 slots 266 us, 188 TFLOP/s of f32-exact products (R = 32, two CTAs of 288 threads an SM): bound
 // by the instructions between the products, about 50 per (slot, row): put three digits together, scale,
 // maximum, exponential, sum, three digits again, add the value sums. Issue slots are 55% busy at 17 warps
 // an SM, which 96 registers a thread allow; the tensor pipe 13%.
@@ -101,6 +101,7 @@ struct KaArgs {
   hg_rows R;
   int nh, g, npb;  // q heads, q heads per kv head, nodes per row block
   int cl;          // CTAs of a unit's cluster, or 0: units on the line
+  int take;        // places on the line for taking a unit up
   const float* q;
   float* out;
   float* part;     // [CTA][2][R * (hd + 2)] partial results: rows of hd sums, then maxima, then sums of p
@@ -201,11 +202,12 @@ __device__ __forceinline__ int ka_tiles(const hg_kv8_cache& C, const SeqSpan& sp
   return (int)((min((long long)sp.start + sp.n, (long long)ka_cap(C)) + KA_TILE - 1) / KA_TILE);
 }
 
-// A unit's length on the line: its tiles and what taking it up costs, about as much as KA_TAKE tiles.
-constexpr int KA_TAKE = 1;
-__device__ __forceinline__ int ka_line(const hg_kv8_cache& C, const SeqSpan& sp) {
-  return ka_tiles(C, sp) + KA_TAKE;
-}
+// A unit's length on the line: its tiles and what taking it up (the digits of its q rows, a first tile
+// with nothing before it, rows written or handed to the join) costs, about as much as `take` tiles.
+// Measured with 1, 2, 3, 4 and 6 places, us: 4 rows, 256 sequences 146.5, 147.8, 148.5, 149.0, 150.5; 16
+// rows, 200 short sequences 79.4, 72.6, 69.8, 70.4, 73.3; 32 rows, wide trees 283, 276, 271, 264, 269.
+constexpr int ka_take(int R) { return R == 4 ? 1 : R == 32 ? 4 : 3; }
+__device__ __forceinline__ int ka_line(const KaArgs& A, const SeqSpan& sp) { return ka_tiles(A.C, sp) + A.take; }
 
 // Row blocks of a sequence.
 __device__ __forceinline__ int ka_blocks(const KaArgs& A, const SeqSpan& sp) {
@@ -223,7 +225,7 @@ __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre
   u.s = a;
   u.sp = kv8_span(A.R, a, true);
   u.tiles = ka_tiles(A.C, u.sp);
-  const int len = A.cl ? 1 : u.tiles + KA_TAKE, blocks = ka_blocks(A, u.sp);
+  const int len = A.cl ? 1 : u.tiles + A.take, blocks = ka_blocks(A, u.sp);
   const int k = A.cl ? t - (int)pre[a] : (int)((uint32_t)(t - (int)pre[a]) / (uint32_t)len);
   u.kvh = blocks == 1 ? k : k / blocks;
   u.blk = k - u.kvh * blocks;
@@ -238,9 +240,9 @@ __device__ __forceinline__ KaPiece ka_piece(const KaArgs& A, const uint32_t* pre
     u.hi = tiles * (rank + 1) / A.cl;
     return u;
   }
-  // the tiles come behind the KA_TAKE places for taking the unit up; a share of those alone is empty
-  u.lo = max(t - u.u0 - KA_TAKE, 0);
-  u.hi = min(end - u.u0 - KA_TAKE, u.tiles);
+  // the tiles come behind the places for taking the unit up; a share of those alone is empty (hi <= lo)
+  u.lo = max(t - u.u0 - A.take, 0);
+  u.hi = min(end - u.u0 - A.take, u.tiles);
   return u;
 }
 // Tiles from here on show nothing to the block's rows.
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
   auto places = [&](int s) -> unsigned long long {
     const SeqSpan sp = kv8_span(A.R, s, true);
     if ((long long)sp.start + sp.n > ka_cap(A.C)) kv8_flag(A.R.err, HG_ERR_CONTEXT);
-    return (unsigned long long)(A.cl ? 1 : ka_line(A.C, sp)) * A.C.n_kv_heads * ka_blocks(A, sp);
+    return (unsigned long long)(A.cl ? 1 : ka_line(A, sp)) * A.C.n_kv_heads * ka_blocks(A, sp);
   };
   auto place32 = [](unsigned long long v) { return (uint32_t)min(v, (unsigned long long)INT_MAX); };
   if (n_seqs > 32) {  // many sequences: every warp loads, then warp 0 adds up
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       const float mine = warp_sums(ls);
       if (lane < RT) sm.wsum[quad][rb + lane] = mine;
       bar_group();
-      const bool from0 = A.cl ? A.cl == 1 : t <= u.u0 + KA_TAKE, to_end = u.next <= end;
+      const bool from0 = A.cl ? A.cl == 1 : t <= u.u0 + A.take, to_end = u.next <= end;
       // where a share's sums go: of a cluster to its own shared memory (the ring is done with)
       float* part = A.cl ? reinterpret_cast<float*>(ka_raw) : A.part + ((size_t)cta * 2 + (from0 ? 1 : 0)) * R * (HD + 2);
       float* out = A.out + ((size_t)(u.sp.r0 + u.j0) * A.nh + u.kvh * A.g) * HD + ti;
@@ -847,13 +849,13 @@ void check_attn(const hg_kv8_cache* c, const hg_rows* r, int n_heads) {
 
 // Rows of a block: 4, 8, 16 or 32, whichever makes a ragged batch cheapest. A block's cost, the mean of
 // the call's time per block at 64 and at 256 rows a kv head (32 sequences of 900 to 7000 slots, 12 q
-// heads, 3 kv heads, 128 dims; us): 11.2, 14.9, 25.6 and 40.4. The whole calls took 723, 466, 391 and 293
-// us at 256 rows, 29.9, 32.1, 36.5 and 53.8 us with the one block that the size just fills. The
+// heads, 3 kv heads, 128 dims; us): 11.7, 13.8, 23.3 and 36.7. The whole calls took 752, 433, 363 and 267
+// us at 256 rows, 31.1, 28.4, 34.0 and 48.0 us with the one block that the size just fills. The
 // sequences' row counts lie between 1 and max_rows; they are taken as spread evenly around their mean.
 int block_rows(const hg_rows* r, int g) {
   const double hi = std::min(r->max_rows, r->n_rows), mean = std::min(hi, (double)r->n_rows / r->n_seqs);
   const double lo = std::min(hi, std::max(1.0, 2 * mean - hi));
-  constexpr double pass[4] = {11.2, 14.9, 25.6, 40.4};
+  constexpr double pass[4] = {11.7, 13.8, 23.3, 36.7};
   double least = 0.0;
   int best = 0;
   for (int i = 0; i < 4; i++) {
@@ -885,7 +887,7 @@ void launch(KaArgs& A, int device, double units, cudaStream_t st) {
   while (cl < KA_CLUSTER && tiles > 2 * cl && units * 2 * cl <= KA_SMS) cl *= 2;
   A.cl = tiles <= 3 * cl && units * cl <= resident ? cl : 0;
   // one CTA per place on the line is the most that can have work
-  const int ctas = A.cl ? (int)units * A.cl : (int)std::min((double)resident, units * (tiles + KA_TAKE));
+  const int ctas = A.cl ? (int)units * A.cl : (int)std::min((double)resident, units * (tiles + A.take));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(S::THREADS);
@@ -939,10 +941,11 @@ extern "C" int hg_op_kv8_attn(const hg_kv8_cache* c, const hg_rows* r, int n_hea
     A.g = n_heads / c->n_kv_heads;
     const int R = block_rows(r, A.g);
     A.npb = R / A.g;
+    A.take = ka_take(R);
     // the most units that ragged rows make; places on the line are numbered with 32 bits
     const double blocks = std::min(std::floor((double)r->n_rows / A.npb) + r->n_seqs,
                                    (double)r->n_seqs * ((std::min(r->max_rows, r->n_rows) + A.npb - 1) / A.npb));
-    const double units = blocks * c->n_kv_heads, places = units * ((c->bt_stride + KA_PAGES - 1) / KA_PAGES + KA_TAKE);
+    const double units = blocks * c->n_kv_heads, places = units * ((c->bt_stride + KA_PAGES - 1) / KA_PAGES + A.take);
     kv8_need(places < 2147483647.0, "rows x table entries x kv heads out of range for one call");
     A.q = q;
     A.out = out;

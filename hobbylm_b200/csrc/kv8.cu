@@ -226,6 +226,9 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
         const float zero[E] = {};
         for (int g = 0; g < count; g++) HeadRow<HD>::store(A.q_out + (row * nh + h0 + g) * HD, zero);
       }
+      // The next fetch writes where this row's copies go, and copies of two groups land in any order: they
+      // are waited for although nobody reads them (a lane's copies always go to the same places).
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
       continue;
     }
     float gain[E], c[H], sn[H];

@@ -2,10 +2,12 @@
 //
 // For a row's q head and the slots t that it sees: p_t = exp(q . k_t / sqrt(hd) - m), out =
 // sum p_t v_t / sum p_t, with k_t = ks_t K_t and v_t = vs_t V_t, K and V int8 codes. Both contractions
-// are integer: q and p_t vs_t are written in fixed point as three signed base-256 digits, so the
-// tensor cores (tcgen05.mma kind::i8) multiply the cache's bytes as they lie in HBM, exactly, and only
-// the rounding to 23 fraction bits of q and of the probabilities (2^-24 of the greatest, what f32
-// rounding costs) and the f32 sums across tiles remain. No code is converted, no K or V value is formed.
+// are integer: q and p_t vs_t are written in fixed point as signed base-256 digits, so the tensor cores
+// (tcgen05.mma kind::i8) multiply the cache's bytes as they lie in HBM, exactly, and only the rounding of
+// q and of the probabilities and the f32 sums across tiles remain. q has four digits, 30 bits from its
+// row's greatest down: with three (23 bits) a q of 1 beside one of 1000 in a channel where K is small would
+// be off by 2^-14. The probabilities have three, 2^-24 of the greatest. No code is converted, no K or V
+// value is formed.
 //
 // A tile is 128 slots (8 pages) of one kv head, and the slots are the MMA's M:
 //   S[slot][digit * R + r] = sum_i K[slot][i] qdigit[r][i]           (A = K pages, B = q digits)
@@ -58,19 +60,20 @@ constexpr float KA_FIX = 8323072.0f;              // 2^23 - 2^16: the greatest f
 // Shared memory of one CTA, in order: the ring, the digits of q and of the probabilities, small arrays.
 template <int HD, int R>
 struct KaShape {
-  static constexpr int N = (3 * R + 15) / 16 * 16;  // MMA N: digit columns
+  static constexpr int NS = 4 * R;                  // MMA N of the scores: columns of q's digits
+  static constexpr int N = (3 * R + 15) / 16 * 16;  // and of the values: columns of the probabilities' digits
   static constexpr int NB = (3 * R + 7) / 8 * 8;    // digit rows kept (what N reads past them stays unread)
   // bytes between 16-byte columns of the digit operands: 16 more than the rows take, so that the two
   // columns that a warp's 32 slots lie in use different banks
-  static constexpr int PITCH = NB * 16 + 16;
+  static constexpr int PITCH_Q = NS * 16 + 16, PITCH = NB * 16 + 16;
   // the rings: V tiles, then K tiles with the scales of both (what a 64-dim V operand reads past its
   // tile, for M = 128, is the next tile)
   static constexpr int VSTAGE = KA_TILE * HD, KSTAGE = VSTAGE + KA_PAGES * 128;
   static constexpr int STAGES = HD == 128 ? 2 : 4;
-  static constexpr int OFF_K = STAGES * VSTAGE, OFF_BQ = OFF_K + STAGES * KSTAGE, OFF_BP = OFF_BQ + PITCH * (HD / 16),
+  static constexpr int OFF_K = STAGES * VSTAGE, OFF_BQ = OFF_K + STAGES * KSTAGE, OFF_BP = OFF_BQ + PITCH_Q * (HD / 16),
                        OFF_SMALL = OFF_BP + PITCH * (KA_TILE / 16);
   // tensor-memory columns: S at 0, O behind it; a power of two of at least 32
-  static constexpr int COL_O = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;
+  static constexpr int COL_O = NS;
   static constexpr int COLS = 2 * COL_O;
   // Compute warps: groups of 128 threads, one slot (S) or dim (O) per thread and RT rows per group; and
   // the copy warp.
@@ -82,10 +85,9 @@ struct KaShape {
 template <int R>
 struct KaSmall {
   uint64_t full_k[4], empty_k[4], full_v[4], empty_v[4], sbar, obar;
-  float wmax[4][R];          // per warp maxima of a tile's scores
-  float wsum[4][R];          // per warp sums at a unit's end
+  float wmax[4][R];          // per warp maxima of a tile's scores, and sums at a unit's end
   float m[2][R];             // running maxima, by the tile's parity
-  float qs[R];               // row r: 256 log2(e) / sqrt(hd) * q scale
+  float qs[R];               // row r: log2(e) / sqrt(hd) * 2^(exponent of its greatest q)
   int lim[R];                // row r sees the slots below, and the tree slots of `vis`; -1: padding
   int node[R], off[R];       // row r's node within its block, its q head's place behind the block's first
   uint32_t vis[R][4];        // slots of the current tile that row r's path holds
@@ -154,19 +156,22 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ void mbar_arrive_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-// A sum whose base-256 digits are d0, d1, d2 (each below 2^21.01 in magnitude). The upper two are put
-// together as integers and converted with one rounding. ka_score drops the lowest 8 of some 30 bits and
-// returns the sum / 256; ka_add adds the sum * f to acc with d0 in full (a dropped part would add up
-// over the tiles).
-__device__ __forceinline__ float ka_score(uint32_t d0, uint32_t d1, uint32_t d2) {
-  return __int2float_rn((int)((d2 << 8) + d1) + ((int)d0 >> 8));
+// Sums whose base-256 digits are d0 .. d3, each below 2^21.01 in magnitude, of two rows, / 65536. The upper
+// two digits are put together as integers and converted with one rounding, d1 + d0 / 256 exactly, and one
+// rounding joins them: like f32 also where the sum is small beside its terms.
+__device__ __forceinline__ f32x2 ka_score(float hi0, float hi1, uint32_t d1, uint32_t e1, uint32_t d0, uint32_t e0) {
+  const f32x2 lo = add2(pack2(__uint_as_float(d1 + (uint32_t)((int)d0 >> 8) + TC_BIAS),
+                              __uint_as_float(e1 + (uint32_t)((int)e0 >> 8) + TC_BIAS)),
+                        pack2(-TC_BIAS_F, -TC_BIAS_F));
+  return fma2(lo, pack2(0.00390625f, 0.00390625f), pack2(hi0, hi1));
 }
+// Adds a sum of three such digits, times f, to acc.
 __device__ __forceinline__ f32x2 ka_add(const uint32_t (&d)[3][2], f32x2 f, f32x2 f256, f32x2 acc) {
   const f32x2 hi = pack2(__int2float_rn((int)((d[2][0] << 8) + d[1][0])), __int2float_rn((int)((d[2][1] << 8) + d[1][1])));
   return fma2(hi, f256, fma2(pack2(__int2float_rn((int)d[0][0]), __int2float_rn((int)d[0][1])), f, acc));
 }
-// Fixed point v (|v| <= KA_FIX) as signed digits v = b0 + 256 b1 + 65536 b2, one per byte.
-__device__ __forceinline__ uint32_t to_digits(uint32_t v) { return (v + 0x808080u) ^ 0x808080u; }
+// Fixed point v (|v| <= 2^30) as signed digits v = b0 + 256 b1 + 65536 b2 + 2^24 b3, one per byte.
+__device__ __forceinline__ uint32_t to_digits(uint32_t v) { return (v + 0x80808080u) ^ 0x80808080u; }
 
 // 8 consecutive tensor-memory columns of this warp's 32 lanes.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
@@ -174,19 +179,53 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                : "r"(taddr));
 }
+// The loads before are over; their registers pass through, so that nothing reads them earlier.
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[N]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
+// The sums of RC rows' scores / 65536, digit i of row r in column i * stride + r (d0 in the first).
+template <int RC>
+__device__ __forceinline__ void tmem_scores(uint32_t t, uint32_t stride, f32x2* s) {
+  uint32_t u[16], v[16];
+  if constexpr (RC == 8) {
+    tmem_ld8(t + 3 * stride, u);
+    tmem_ld8(t + 2 * stride, u + 8);
+    tmem_wait(u);
+    tmem_ld8(t + stride, v);
+    tmem_ld8(t, v + 8);
+  } else {
+    tmem_ld16(t, v);  // the stride is 4: one read has them all
+    tmem_wait(v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i] = v[12 + i], u[4 + i] = v[8 + i];
+  }
+  float hi[RC];
+#pragma unroll
+  for (int r = 0; r < RC; r++) hi[r] = __int2float_rn((int)((u[r] << 8) + u[RC + r]));
+  if constexpr (RC == 8) tmem_wait(v);
+  const uint32_t *d1 = RC == 8 ? v : v + 4, *d0 = RC == 8 ? v + 8 : v;
+#pragma unroll
+  for (int r = 0; r < RC; r += 2) s[r / 2] = ka_score(hi[r], hi[r + 1], d1[r], d1[r + 1], d0[r], d0[r + 1]);
+}
 // The three digit columns of RC rows: digit i of row r is column i * stride + r.
 template <int RC>
 __device__ __forceinline__ void tmem_rows(uint32_t t, uint32_t stride, uint32_t (&d)[3][RC]) {
   if constexpr (RC == 8) {
 #pragma unroll
     for (int i = 0; i < 3; i++) tmem_ld8(t + i * stride, d[i]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 24; i++) asm volatile("" : "+r"(d[i / 8][i % 8]));
   } else {
     uint32_t v[16];  // the stride is RC: one read has them all
     tmem_ld16(t, v);
+    tmem_wait(v);
 #pragma unroll
     for (int i = 0; i < 3 * RC; i++) d[i / RC][i % RC] = v[i];
   }
-  tmem_ld_wait();
 }
 
 // A run of tiles of one unit, as both the copy warp and the compute warps walk it.
@@ -410,14 +449,14 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       else bar_named<128>(2 + grp);
     };
     const uint32_t bq_a = smem_u32(bq), bp_a = smem_u32(bp), ring_a = smem_u32(ka_raw);
-    constexpr uint32_t IDESC = tc_idesc(KA_TILE, S::N);
+    constexpr uint32_t IDESC_S = tc_idesc(KA_TILE, S::NS), IDESC_O = tc_idesc(KA_TILE, S::N);
     int n = 0;  // tiles done by this CTA
     auto issue_scores = [&](int k) {  // thread 0: S = K . q digits
       const uint32_t a = ring_a + S::OFF_K + k * S::KSTAGE;
 #pragma unroll
       for (int i = 0; i < HD / 32; i++)
-        tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::PITCH, S::PITCH, 128, 0),
-                   IDESC, i > 0);
+        tc_mma_acc(tm, tc_desc(a + i * 256, 128, 8 * HD, 0), tc_desc(bq_a + i * 2 * S::PITCH_Q, S::PITCH_Q, 128, 0),
+                   IDESC_S, i > 0);
       tc_commit(&sm.sbar);
     };
     for (int t = begin; t < end;) {
@@ -463,26 +502,28 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           poison = __fmaf_rn(x[i][e], 0.0f, poison);  // NaN for a NaN or an infinity
         }
         amax = warp_fmax(amax);
-        const float inv = amax > 1e-30f ? __fdiv_rn(KA_FIX, amax) : 0.0f;  // below: the scores are zero
-        uint32_t w[3] = {0, 0, 0};
+        // units of 2^(ex - 29), so that |v| < 2^30: a power of two, so that what lies within 2^6 of the greatest is exact
+        const int ex = min(max((int)(__float_as_uint(amax) >> 23) - 127, -97), 127);
+        const float inv = __uint_as_float((uint32_t)(156 - ex) << 23);
+        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < E; e++) {
-          const uint32_t d = to_digits((uint32_t)__float2int_rn(fminf(fmaxf(x[i][e] * inv, -KA_FIX), KA_FIX)));
+          const uint32_t d = to_digits((uint32_t)__float2int_rn(x[i][e] * inv));
 #pragma unroll
-          for (int b = 0; b < 3; b++) w[b] |= ((d >> (8 * b)) & 255u) << (8 * e);
+          for (int b = 0; b < 4; b++) w[b] |= ((d >> (8 * b)) & 255u) << (8 * e);
         }
 #pragma unroll
-        for (int b = 0; b < 3; b++) {
+        for (int b = 0; b < 4; b++) {
           const int row = b * R + r, kb = lane * E;
-          unsigned char* d = bq + (kb >> 4) * S::PITCH + (row >> 3) * 128 + (row & 7) * 16 + (kb & 15);
+          unsigned char* d = bq + (kb >> 4) * S::PITCH_Q + (row >> 3) * 128 + (row & 7) * 16 + (kb & 15);
           if constexpr (E == 4) *reinterpret_cast<uint32_t*>(d) = w[b];
           else *reinterpret_cast<uint16_t*>(d) = (uint16_t)w[b];
         }
         const bool bad = __any_sync(0xffffffffu, poison != poison);
-        // never zero: the -infinity of a masked slot has to stay one
+        // (never zero: the -infinity of a masked slot has to stay one)
         if (lane == 0)
           sm.qs[r] = bad ? __int_as_float(0x7fffffff)
-                         : fmaxf((float)((double)amax * (256.0 * 1.4426950408889634 / 8323072.0 / sqrt((double)HD))), 1e-37f);
+                         : (float)(1.4426950408889634 / (HD == 64 ? 8.0 : 11.313708498984761)) * __uint_as_float((uint32_t)(ex + 127) << 23);
       }
       fence_async_smem();
       bar_all();
@@ -554,14 +595,13 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         __syncwarp();
         tc_fence_after();
         f32x2 s[RT / 2];
-        const f32x2 ks2 = pack2(ks, ks);
+        const float ks13 = ks * 0.0001220703125f;  // 2^-13: 2^-29 of q's units, 2^16 of the sums'
+        const f32x2 ks2 = pack2(ks13, ks13);
 #pragma unroll
         for (int r0 = 0; r0 < RT; r0 += S::RC) {
-          uint32_t d[3][S::RC];
-          tmem_rows<S::RC>(tq + r0, R, d);
+          tmem_scores<S::RC>(tq + r0, R, s + r0 / 2);
 #pragma unroll
-          for (int r = 0; r < S::RC; r += 2)
-            s[(r0 + r) / 2] = mul2(pack2(ka_score(d[0][r], d[1][r], d[2][r]), ka_score(d[0][r + 1], d[1][r + 1], d[2][r + 1])), ks2);
+          for (int r = 0; r < S::RC; r += 2) s[(r0 + r) / 2] = mul2(s[(r0 + r) / 2], ks2);
         }
         if (!whole) {
           const bool in = (there >> (ti >> 4)) & 1u;
@@ -659,7 +699,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
 #pragma unroll
           for (int i = 0; i < KA_TILE / 32; i++)
             tc_mma_acc(tm + S::COL_O, tc_desc(a + i * 32 * HD, 16 * HD, 128, 0),
-                       tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC, i > 0);
+                       tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC_O, i > 0);
           tc_commit(&sm.obar);
           if (tile + 1 < last) {  // the next tile's scores meanwhile
             ka_wait(&sm.full_k[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
@@ -677,7 +717,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         unpack2(acc[r / 2], sums[r], sums[r + 1]);
       }
       const float mine = warp_sums(ls);
-      if (lane < RT) sm.wsum[quad][rb + lane] = mine;
+      if (lane < RT) sm.wmax[quad][rb + lane] = mine;
       bar_group();
       const bool from0 = A.cl ? A.cl == 1 : t <= u.u0 + A.take, to_end = u.next <= end;
       // where a share's sums go: of a cluster to its own shared memory (the ring is done with)
@@ -686,7 +726,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
 #pragma unroll
       for (int r = 0; r < RT; r++) {
         const int row = rb + r;
-        float tot = (sm.wsum[0][row] + sm.wsum[1][row]) + (sm.wsum[2][row] + sm.wsum[3][row]);
+        float tot = (sm.wmax[0][row] + sm.wmax[1][row]) + (sm.wmax[2][row] + sm.wmax[3][row]);
         if (sm.lim[row] < 0) tot = 0.0f;
         if (from0 && to_end) {
           if (sm.node[row] < u.nodes && ti < HD) out[sm.off[row] * HD] = tot == 0.0f ? 0.0f : __fdiv_rn(sums[r], tot);

@@ -67,3 +67,103 @@ def test_append_between_padding_rows(native, heads):
             assert np.array_equal(codes[i], wc)
             assert np.array_equal(codes[2][:, :, i].view(np.int32), ws.view(np.int32))
     assert b.err_code() == CONTEXT
+
+
+# ---------------------------------------------------------------------------------------------
+# attention at any spread of scales
+# ---------------------------------------------------------------------------------------------
+def _attend(q, kc, vc, ks, vs, b, f32=False):
+    """Attention in 64 bits with a bound on the kernel's error, and (f32) the plain 32-bit form beside it.
+
+    The bound, from what the kernel rounds, for a row that sees n slots in T tiles, with x its scores:
+    * the joined sums, K scale, q scale, and the sum with the V scale's exponent: 5 roundings of |x|, 3 of
+      the exponent in log2 units (its rounding, the difference to the maximum, that maximum in the join);
+      exp2: 2 ulp. A row's maximum changes at most T + 2 times (its tiles, the join), each an exp2.
+    * q: fixed point, off by 2^-30 of its greatest value at most, each dim's with a sign of its own: eight
+      of the greatest deviations over dims and slots (Hoeffding: 1e-13).
+    * a product p v_scale: half a unit, 2^-22 / (1 - 2^-7) of the greatest; the roundings of n slots have
+      independent signs (the codes' are random): eight of the greatest deviations.
+    * f32 sums: four roundings a tile, and 40 for the warps' and the shares' sums and the quotients."""
+    n, nh, hd = q.shape
+    g = nh // b.nkv
+    out, tol, plain = np.zeros((n, nh, hd)), np.zeros((n, nh, hd)), np.zeros((n, nh, hd), np.float32)
+    for s in range(len(b.starts)):
+        for r in range(b.row_off[s], b.row_off[s + 1]):
+            path = kv.path_of(b.parent, b.row_off[s], r - b.row_off[s])
+            slots = np.concatenate([np.arange(b.starts[s]), b.starts[s] + np.array(path)]).astype(np.int64)
+            if not path:
+                continue
+            page, w = b.table[s, slots // PAGE], slots % PAGE
+            tiles = int(slots.max()) // 128 + 1
+            for h in range(nh):
+                i = h // g
+                kk, vv = (c[page, i, w].astype(np.float64) * sc[page, i, w][:, None].astype(np.float64) for c, sc in ((kc, ks), (vc, vs)))
+                qq = q[r, h].astype(np.float64)
+                x = kk @ qq / np.sqrt(hd)
+                p = np.exp(x - x.max())
+                out[r, h] = p @ vv / p.sum()
+                scale = vs[page, i, w].astype(np.float64)
+                e = np.maximum(np.floor(np.log2(np.maximum(scale, 1e-300))), -60)
+                top = np.abs(x).max()
+                rel = U * (5 * top + 3 * (1.45 * top + np.abs(e).max() + 1) + 5) + 5 * U * (tiles + 2)
+                step = 2.0 ** -30 * np.abs(qq).max() / np.sqrt(hd)  # of q, as a score takes it
+                pk = p * np.sqrt((kk * kk).sum(1))
+                q_off = 8 * step * (np.sqrt(pk ** 2 @ vv ** 2) + np.sqrt((pk ** 2).sum()) * np.abs(out[r, h]))
+                size = p @ np.abs(vv)
+                most = (p * np.maximum(scale, 2.0 ** -60)).max()
+                codes = np.sqrt((vc[page, i, w].astype(np.float64) ** 2).sum(0))
+                unit = most * 2.0 ** -22 / (1 - 2.0 ** -7)
+                tol[r, h] = (size * (2 * rel + (4 * tiles + 40) * U) + 8 * codes * unit / 2 + q_off) / p.sum()
+                if f32:
+                    x4 = (kk.astype(np.float32) @ q[r, h]) * np.float32(1 / np.sqrt(hd))
+                    p4 = np.exp(x4 - x4.max())
+                    plain[r, h] = p4 @ vv.astype(np.float32) / p4.sum()
+    return (out, tol, plain) if f32 else (out, tol)
+
+
+def _scaled_pool(b, rng, change):
+    """Random codes, scales changed by change(scales [page][head][32], K codes, V codes), uploaded."""
+    b.fill(rng)
+    pool = b.pool_np().copy()
+    k_at, v_at = kv.block_index(b.hd)
+    kc, vc = (np.ascontiguousarray(pool.view(np.int8)[..., at]) for at in (k_at, v_at))
+    sc = np.ascontiguousarray(pool[..., 32 * b.hd:]).view(np.float32).copy()
+    change(sc, kc, vc)
+    pool.view(np.int8)[..., k_at], pool.view(np.int8)[..., v_at] = kc, vc
+    pool[..., 32 * b.hd:] = sc.view(np.uint8)
+    full = np.zeros((b.n_pages, b.stride), np.uint8)
+    full[:, :b.nkv * b.block] = pool.reshape(b.n_pages, -1)
+    b.pool.copy_(kv.dev(full.reshape(-1)))
+    return kc, vc, sc[..., :16], sc[..., 16:]
+
+
+def _check_scales(b, rng, change, q=None):
+    kc, vc, ks, vs = _scaled_pool(b, rng, change)
+    q = rng.standard_normal((b.n, b.nh, b.hd)).astype(np.float32) if q is None else q
+    out = b.attn(q).cpu().numpy().reshape(-1, b.nh, b.hd)
+    want, tol, plain = _attend(q, kc, vc, ks, vs, b, True)
+    size = np.sqrt((want ** 2).mean(-1, keepdims=True)) + 1e-300
+    live = (want != 0).any((1, 2))
+    rms = [np.sqrt((((y - want) / size)[live] ** 2).mean()) for y in (out, plain)]
+    print(f"relative error, root mean square: kernel {rms[0]:.1e}, plain f32 {rms[1]:.1e}")
+    bad = ~(np.abs(out - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:3], rms)
+    assert (out[~live] == 0).all() and b.err_code() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("factor", [30.0, 300.0, 5000.0])
+def test_attn_channels_of_unequal_size(native, hd, factor):
+    """K's great channels stand where q is small, q's where K is: neither takes the others' accuracy."""
+    rng = np.random.default_rng(55)
+    b = kv.Batch(native, rng, (4, 1, hd), [900], [3])
+    q = rng.standard_normal((b.n, 4, hd)).astype(np.float32)
+    q[..., 5] *= np.float32(factor)
+    q[..., 20] /= np.float32(factor)
+
+    def change(sc, kc, vc):
+        kc[..., 5] = 0
+        kc[..., 20] = np.where(rng.random(kc[..., 20].shape) < 0.5, 127, -127)
+
+    _check_scales(b, rng, change, q)

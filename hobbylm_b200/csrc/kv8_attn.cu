@@ -6,8 +6,17 @@
 // (tcgen05.mma kind::i8) multiply the cache's bytes as they lie in HBM, exactly, and only the rounding of
 // q and of the probabilities and the f32 sums across tiles remain. q has four digits, 30 bits from its
 // row's greatest down: with three (23 bits) a q of 1 beside one of 1000 in a channel where K is small would
-// be off by 2^-14. The probabilities have three, 2^-24 of the greatest. No code is converted, no K or V
-// value is formed.
+// be off by 2^-14. No code is converted, no K or V value is formed.
+//
+// The values' digits have to hold p_t vs_t and not p_t: what a slot adds goes by both, and the greatest p
+// and the greatest vs may stand in different slots, or the latter where only another row sees it. So with
+// vs_t = 2^e_t f_t, f_t from 1 to 2, a row's running maximum is that of y_t = log2 p_t + e_t (e_t an integer,
+// so that nothing is lost by putting it there), the digits are those of 2^(y_t - max) f_t, three of them,
+// 2^-23 of the row's own greatest product, and the sum of p takes 2^(y_t - max) 2^-e_t, exact powers of
+// two. e_t is -60 at least: V scales below 2^-60, zeros among them, count with f_t < 1. Measured against
+// 64-bit attention over the same codes, V scales equal, spread lognormally (sigma 1 and 3), or with one in
+// 100 being 100 or 1000 times the rest, seen by a row or not: off by 3e-7 to 1.3e-6 (root mean square,
+// relative), plain f32 arithmetic by 2e-7 to 9e-7.
 //
 // A tile is 128 slots (8 pages) of one kv head, and the slots are the MMA's M:
 //   S[slot][digit * R + r] = sum_i K[slot][i] qdigit[r][i]           (A = K pages, B = q digits)
@@ -33,8 +42,8 @@
 //
 // Measured: 256 sequences of 1024 to 8192 slots (12 q heads, 3 kv heads, 128 dims) 147-152 us, 5.9 TB/s
 // of cache, 0.90 of measured HBM (R = 4, three CTAs an SM: bound by HBM). 32 trees of 64 nodes over 900
-// to 7000 slots 266 us, 188 TFLOP/s of f32-exact products (R = 32, two CTAs of 288 threads an SM): bound
-// by the instructions between the products, about 50 per (slot, row): put three digits together, scale,
+// to 7000 slots 264 us, 190 TFLOP/s of f32-like products (R = 32, two CTAs of 288 threads an SM): bound
+// by the instructions between the products, about 50 per (slot, row): put four digits together, scale,
 // maximum, exponential, sum, three digits again, add the value sums. Issue slots are 55% busy at 17 warps
 // an SM, which 96 registers a thread allow; the tensor pipe 13%.
 #include <cooperative_groups.h>
@@ -54,8 +63,9 @@ constexpr int KA_PAGES = KA_TILE / KV8_PAGE;      // pages of a tile
 constexpr int KA_SMS = 148;
 constexpr int KA_MAX_CTAS = 3 * KA_SMS;
 constexpr int KA_CLUSTER = 16;                    // most CTAs of a unit's cluster
-constexpr float KA_NONE = -1e30f;                 // maximum of a row that has seen nothing: finite, below any score
+constexpr float KA_NONE = -3e38f;                 // maximum of a row that has seen nothing: finite, below any score
 constexpr float KA_FIX = 8323072.0f;              // 2^23 - 2^16: the greatest fixed-point value, three digits
+constexpr float KA_UNIT = 2.0f / KA_FIX;          // a unit of the probabilities' digits
 
 // Shared memory of one CTA, in order: the ring, the digits of q and of the probabilities, small arrays.
 template <int HD, int R>
@@ -86,12 +96,11 @@ template <int R>
 struct KaSmall {
   uint64_t full_k[4], empty_k[4], full_v[4], empty_v[4], sbar, obar;
   float wmax[4][R];          // per warp maxima of a tile's scores, and sums at a unit's end
-  float m[2][R];             // running maxima, by the tile's parity
+  float m[2][R];             // running maxima of score + exponent of the V scale (log2), by the tile's parity
   float qs[R];               // row r: log2(e) / sqrt(hd) * 2^(exponent of its greatest q)
   int lim[R];                // row r sees the slots below, and the tree slots of `vis`; -1: padding
   int node[R], off[R];       // row r's node within its block, its q head's place behind the block's first
   uint32_t vis[R][4];        // slots of the current tile that row r's path holds
-  float wsv[2][4];
   uint32_t pages[4];         // per stage: which of the tile's pages are there
   uint32_t tmem;
   int fail;
@@ -107,7 +116,7 @@ struct KaArgs {
   const float* q;
   float* out;
   float* part;     // [CTA][2][R * (hd + 2)] partial results: rows of hd sums, then maxima, then sums of p
-  int4* head;      // [CTA][2] of the joins: {sequence, kv head * 65536.. (see k_kv8_join)}
+  int4* head;      // [CTA] of a join: first row (-1: none), kv head, nodes, the CTA of the unit's last place
 };
 
 // Two rows' f32 values side by side: one instruction for both.
@@ -165,10 +174,10 @@ __device__ __forceinline__ f32x2 ka_score(float hi0, float hi1, uint32_t d1, uin
                         pack2(-TC_BIAS_F, -TC_BIAS_F));
   return fma2(lo, pack2(0.00390625f, 0.00390625f), pack2(hi0, hi1));
 }
-// Adds a sum of three such digits, times f, to acc.
-__device__ __forceinline__ f32x2 ka_add(const uint32_t (&d)[3][2], f32x2 f, f32x2 f256, f32x2 acc) {
+// Adds sums of three such digits to acc.
+__device__ __forceinline__ f32x2 ka_add(const uint32_t (&d)[3][2], f32x2 acc) {
   const f32x2 hi = pack2(__int2float_rn((int)((d[2][0] << 8) + d[1][0])), __int2float_rn((int)((d[2][1] << 8) + d[1][1])));
-  return fma2(hi, f256, fma2(pack2(__int2float_rn((int)d[0][0]), __int2float_rn((int)d[0][1])), f, acc));
+  return fma2(hi, pack2(256.0f, 256.0f), add2(pack2(__int2float_rn((int)d[0][0]), __int2float_rn((int)d[0][1])), acc));
 }
 // Fixed point v (|v| <= 2^30) as signed digits v = b0 + 256 b1 + 65536 b2 + 2^24 b3, one per byte.
 __device__ __forceinline__ uint32_t to_digits(uint32_t v) { return (v + 0x80808080u) ^ 0x80808080u; }
@@ -520,7 +529,6 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           else *reinterpret_cast<uint16_t*>(d) = (uint16_t)w[b];
         }
         const bool bad = __any_sync(0xffffffffu, poison != poison);
-        // (never zero: the -infinity of a masked slot has to stay one)
         if (lane == 0)
           sm.qs[r] = bad ? __int_as_float(0x7fffffff)
                          : (float)(1.4426950408889634 / (HD == 64 ? 8.0 : 11.313708498984761)) * __uint_as_float((uint32_t)(ex + 127) << 23);
@@ -528,7 +536,6 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       fence_async_smem();
       bar_all();
       f32x2 acc[RT / 2], l[RT / 2];
-      float c_run = 0.0f, of = 0.0f;
 #pragma unroll
       for (int r = 0; r < RT / 2; r++) acc[r] = l[r] = 0ull;
       // the sums over the dims that the MMAs of tile n - 1 left in tensor memory
@@ -537,7 +544,6 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         __syncwarp();
         tc_fence_after();
         if (tid == 0) mbar_arrive(&sm.empty_v[n_of % STAGES]);
-        const f32x2 f = pack2(of, of), f256 = pack2(of * 256.0f, of * 256.0f);
 #pragma unroll
         for (int r0 = 0; r0 < RT; r0 += S::RC) {
           uint32_t d[3][S::RC];
@@ -545,7 +551,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
 #pragma unroll
           for (int r = 0; r < S::RC; r += 2) {
             const uint32_t e[3][2] = {{d[0][r], d[0][r + 1]}, {d[1][r], d[1][r + 1]}, {d[2][r], d[2][r + 1]}};
-            acc[(r0 + r) / 2] = ka_add(e, f, f256, acc[(r0 + r) / 2]);
+            acc[(r0 + r) / 2] = ka_add(e, acc[(r0 + r) / 2]);
           }
         }
         tc_fence_before();
@@ -561,8 +567,13 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         ka_wait(&sm.full_k[k], (n / STAGES) & 1, &sm.fail);  // the scales (the codes are the MMAs')
         const float* sc =
             reinterpret_cast<const float*>(ka_raw + S::OFF_K + k * S::KSTAGE + S::VSTAGE + (ti >> 4) * 128) + (ti & 15);
-        const float ks = sc[0];
-        float vs = sc[16];
+        // the V scale as 2^e times 1 to 2 (below 2^-60, or 0: times less than 1); a NaN, an infinity or what is
+        // below zero is nothing, and poisons the rows that see the slot
+        const float ks = fabsf(sc[0]) <= 3.402823466e38f ? sc[0] : __int_as_float(0x7fffffff), vs = sc[16];
+        const bool fine = vs >= 0.0f && vs < 1.7014118346e38f;
+        const uint32_t ve = fine ? max((__float_as_uint(vs) & 0x7fffffffu) >> 23, 67u) : 127u;
+        const float e = (float)((int)ve - 127), inv = __uint_as_float((254u - ve) << 23);
+        const float pf = fine ? vs * inv * (KA_FIX * 0.5f) : 0.0f;
         const uint32_t there = sm.pages[k];
         // every slot is context of every row and its page is there: nothing to mask
         const bool whole = there == (1u << KA_PAGES) - 1 && (tile + 1) * KA_TILE <= u.sp.start;
@@ -596,16 +607,20 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         tc_fence_after();
         f32x2 s[RT / 2];
         const float ks13 = ks * 0.0001220703125f;  // 2^-13: 2^-29 of q's units, 2^16 of the sums'
-        const f32x2 ks2 = pack2(ks13, ks13);
+        const f32x2 ks2 = pack2(ks13, ks13), e2 = pack2(e, e);
 #pragma unroll
         for (int r0 = 0; r0 < RT; r0 += S::RC) {
           tmem_scores<S::RC>(tq + r0, R, s + r0 / 2);
 #pragma unroll
-          for (int r = 0; r < S::RC; r += 2) s[(r0 + r) / 2] = mul2(s[(r0 + r) / 2], ks2);
+          for (int r = 0; r < S::RC; r += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(&sm.qs[rb + r0 + r]);
+            f32x2* x = s + (r0 + r) / 2;
+            x[0] = fma2(mul2(x[0], ks2), pack2(q.x, q.y), e2);
+            x[1] = fma2(mul2(x[1], ks2), pack2(q.z, q.w), e2);
+          }
         }
         if (!whole) {
           const bool in = (there >> (ti >> 4)) & 1u;
-          bool any = false;
 #pragma unroll
           for (int r = 0; r < RT; r += 2) {
             float x[2];
@@ -614,14 +629,12 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             for (int i = 0; i < 2; i++) {
               bool see = slot < sm.lim[rb + r + i];
               if (tree) see = see || ((sm.vis[rb + r + i][quad] >> lane) & 1u);
-              if (see && in) any = true;
-              else x[i] = -INFINITY;
+              if (!(see && in)) x[i] = -INFINITY;
             }
             s[r / 2] = pack2(x[0], x[1]);
           }
-          if (!any) vs = 0.0f;  // what lies in an unseen slot counts nowhere, not for the scales' maximum either
         }
-        // ---- the tile's maximum per row (a row's scale is left out until the exponent), and of the V scales ----
+        // ---- the tile's maximum per row ----
 #pragma unroll
         for (int r = 0; r < RT; r += 4) {
           float x[4];
@@ -630,16 +643,11 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           const float4 v = make_float4(warp_fmax(x[0]), warp_fmax(x[1]), warp_fmax(x[2]), warp_fmax(x[3]));
           if (lane == 0) *reinterpret_cast<float4*>(&sm.wmax[quad][rb + r]) = v;
         }
-        const float vfin = vs <= 3.402823466e38f ? vs : 0.0f;
-        const float vm = warp_fmax(vfin);
-        if (lane == 0) sm.wsv[grp][quad] = vm;
         if (tile > u.lo) add_out(n - 1);  // the previous tile's sums, while the others get here
         bar_group();
-        c_run = fmaxf(fmaxf(c_run, fmaxf(sm.wsv[grp][0], sm.wsv[grp][1])), fmaxf(sm.wsv[grp][2], sm.wsv[grp][3]));
-        const float pf = c_run > 0.0f ? __fdiv_rn(vfin, c_run) * KA_FIX : 0.0f;
         const int now = n & 1;
-        if (__any_sync(0xffffffffu, vs != vfin)) {  // a NaN or infinite V scale poisons the rows that see the slot
-          const float bad = vs != vfin ? __int_as_float(0x7fffffff) : 0.0f;
+        if (__any_sync(0xffffffffu, !fine)) {
+          const float bad = fine ? 0.0f : __int_as_float(0x7fffffff);
 #pragma unroll
           for (int r = 0; r < RT; r += 2) {
             float x[2];
@@ -647,19 +655,18 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             l[r / 2] = add2(l[r / 2], pack2(x[0] != -INFINITY ? bad : 0.0f, x[1] != -INFINITY ? bad : 0.0f));
           }
         }
-        const f32x2 pf2 = pack2(pf, pf), minus1 = pack2(-1.0f, -1.0f), big = pack2(8388608.0f + 32896.0f, 8388608.0f + 32896.0f);
+        const f32x2 pf2 = pack2(pf, pf), inv2 = pack2(inv, inv), big = pack2(8388608.0f + 32896.0f, 8388608.0f + 32896.0f);
 #pragma unroll
         for (int r0 = 0; r0 < RT; r0 += 4) {  // four rows at a time, so that their maxima need not stay in registers
           const float4 a = *reinterpret_cast<const float4*>(&sm.wmax[0][rb + r0]), b = *reinterpret_cast<const float4*>(&sm.wmax[1][rb + r0]);
           const float4 c = *reinterpret_cast<const float4*>(&sm.wmax[2][rb + r0]), d = *reinterpret_cast<const float4*>(&sm.wmax[3][rb + r0]);
-          const float4 o = *reinterpret_cast<const float4*>(&sm.m[now ^ 1][rb + r0]), q4 = *reinterpret_cast<const float4*>(&sm.qs[rb + r0]);
+          const float4 o = *reinterpret_cast<const float4*>(&sm.m[now ^ 1][rb + r0]);
           const float4 m4 = make_float4(fmaxf(fmaxf(fmaxf(a.x, b.x), fmaxf(c.x, d.x)), o.x), fmaxf(fmaxf(fmaxf(a.y, b.y), fmaxf(c.y, d.y)), o.y),
                                         fmaxf(fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z)), o.z), fmaxf(fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w)), o.w));
           if (ti == 0) *reinterpret_cast<float4*>(&sm.m[now][rb + r0]) = m4;
-          const float m[4] = {m4.x, m4.y, m4.z, m4.w}, q[4] = {q4.x, q4.y, q4.z, q4.w};
+          const float m[4] = {m4.x, m4.y, m4.z, m4.w};
           if (m[0] > o.x || m[1] > o.y || m[2] > o.z || m[3] > o.w) {  // the same for every thread of the group
-            const f32x2 al[2] = {pack2(ex2((o.x - m[0]) * q[0]), ex2((o.y - m[1]) * q[1])),
-                                 pack2(ex2((o.z - m[2]) * q[2]), ex2((o.w - m[3]) * q[3]))};
+            const f32x2 al[2] = {pack2(ex2(o.x - m[0]), ex2(o.y - m[1])), pack2(ex2(o.z - m[2]), ex2(o.w - m[3]))};
 #pragma unroll
             for (int i = 0; i < 2; i++) {
               acc[r0 / 2 + i] = mul2(acc[r0 / 2 + i], al[i]);
@@ -669,9 +676,9 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
 #pragma unroll
           for (int r = r0; r < r0 + 4; r += 2) {
             float x[2];
-            unpack2(mul2(fma2(pack2(m[r - r0], m[r - r0 + 1]), minus1, s[r / 2]), pack2(q[r - r0], q[r - r0 + 1])), x[0], x[1]);
+            unpack2(add2(s[r / 2], pack2(-m[r - r0], -m[r - r0 + 1])), x[0], x[1]);
             const f32x2 p = pack2(ex2(x[0]), ex2(x[1]));
-            l[r / 2] = add2(l[r / 2], p);
+            l[r / 2] = fma2(p, inv2, l[r / 2]);
             // p * pf in [0, KA_FIX], rounded into the low bits of 2^23 + 0x8080 + v: the lower digits' bytes
             // are 128 up, which the exclusive or takes back
             unpack2(fma2(p, pf2, big), x[0], x[1]);
@@ -687,7 +694,6 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             }
           }
         }
-        of = c_run * (1.0f / KA_FIX);
         fence_async_smem();
         tc_fence_before();
         bar_all();
@@ -729,11 +735,11 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         float tot = (sm.wmax[0][row] + sm.wmax[1][row]) + (sm.wmax[2][row] + sm.wmax[3][row]);
         if (sm.lim[row] < 0) tot = 0.0f;
         if (from0 && to_end) {
-          if (sm.node[row] < u.nodes && ti < HD) out[sm.off[row] * HD] = tot == 0.0f ? 0.0f : __fdiv_rn(sums[r], tot);
+          if (sm.node[row] < u.nodes && ti < HD) out[sm.off[row] * HD] = tot == 0.0f ? 0.0f : __fdiv_rn(sums[r] * KA_UNIT, tot);
         } else {
           if (ti < HD) part[row * HD + ti] = sums[r];
           if (ti == 0) {
-            part[R * HD + row] = sm.m[(n + 1) & 1][row] * sm.qs[row];
+            part[R * HD + row] = sm.m[(n + 1) & 1][row];
             part[R * HD + R + row] = tot;
           }
         }
@@ -775,7 +781,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           o = __fmaf_rn(v[c], f, o);
           tot = __fmaf_rn(l[c], f, tot);
         }
-        A.out[((size_t)sm.first_row * A.nh + sm.kvh * A.g + sm.off[r]) * HD + i] = tot == 0.0f ? 0.0f : __fdiv_rn(o, tot);
+        A.out[((size_t)sm.first_row * A.nh + sm.kvh * A.g + sm.off[r]) * HD + i] = tot == 0.0f ? 0.0f : __fdiv_rn(o * KA_UNIT, tot);
       }
     }
     cg::this_cluster().sync();  // nobody leaves while its shared memory is read
@@ -842,7 +848,7 @@ __global__ void __launch_bounds__(KA_STRANDS * 32) k_kv8_join(const __grid_const
   auto put = [&](int r, Dims o, float tot) {
     const int node = r / A.g;
 #pragma unroll
-    for (int e = 0; e < E; e++) o.d[e] = tot == 0.0f ? 0.0f : __fdiv_rn(o.d[e], tot);
+    for (int e = 0; e < E; e++) o.d[e] = tot == 0.0f ? 0.0f : __fdiv_rn(o.d[e] * KA_UNIT, tot);
     reinterpret_cast<Dims*>(A.out + ((size_t)(h.x + node) * A.nh + h.y * A.g + r - node * A.g) * HD)[i] = o;
   };
   const int have = h.z * A.g;  // rows of the block

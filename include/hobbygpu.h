@@ -338,7 +338,7 @@ int hg_op_kv_attn(const hg_kv_attn_args* a, void* scratch, void* stream);
  *   K codes, int8, at (w / 8) * 8 * head_dim + (i / 16) * 128 + (w % 8) * 16 + i % 16
  *   V codes, int8, at 16 * head_dim + i * 16 + w
  *   K scales, f32 [16], at 32 * head_dim, and V scales, f32 [16], at 32 * head_dim + 64
- * A value is code * scale, |code| <= 127; a row with a NaN or an infinity has scale NaN. */
+ * A value is code * scale, |code| <= 127, scale >= 0; a row with a NaN or an infinity has scale NaN. */
 typedef struct {
   int32_t n_kv_heads, head_dim;  /* head_dim 64 or 128 */
   int32_t n_pages;               /* pages of the pool: a table entry outside 0..n_pages-1 is no page */
@@ -391,7 +391,11 @@ int hg_op_kv8_read(const hg_kv8_cache* c, const hg_rows* r, float* k_out, float*
 /* Attention of every row's q heads (normed and roped, as hg_op_kv8_append writes them) over the slots it
  * sees: 0..start[s]-1, its ancestors' and its own (the rows are in the cache already), softmax of
  * q . k / sqrt(head_dim). q, out: [n_rows][n_heads * head_dim] f32, n_heads / n_kv_heads at most 32.
- * Slots without a page are not seen (err HG_ERR_CONTEXT); a row that sees nothing gets zeros. scratch:
+ * Slots without a page are not seen (err HG_ERR_CONTEXT); a row that sees nothing gets zeros; one that sees
+ * a scale that is NaN or infinite, or a V scale below zero or from 2^127 up, gets NaN. A q value counts to
+ * 2^-30 of its row's greatest, a probability times its V scale to 2^-23 of the greatest that the row sees,
+ * all else as in f32, at any spread of V scales from 2^-60 to 2^60 and zero (what is below 2^-60 counts to
+ * 2^-83 absolutely). scratch:
  * 16-byte aligned device buffer of hg_op_kv8_attn_scratch_bytes() bytes (the same for every batch of one
  * head_dim), its content of no meaning before and after the call; calls that may overlap need one each. */
 size_t hg_op_kv8_attn_scratch_bytes(const hg_kv8_cache* c, const hg_rows* r, int n_heads);

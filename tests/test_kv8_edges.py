@@ -167,3 +167,104 @@ def test_attn_channels_of_unequal_size(native, hd, factor):
         kc[..., 20] = np.where(rng.random(kc[..., 20].shape) < 0.5, 127, -127)
 
     _check_scales(b, rng, change, q)
+
+
+SPREADS = {
+    "sigma 1": lambda sc, rng: np.exp(rng.standard_normal(sc.shape)) * 0.02,
+    "sigma 3": lambda sc, rng: np.where(np.arange(32) < 16, sc, np.exp(3 * rng.standard_normal(sc.shape)) * 0.02),
+    "tiny": lambda sc, rng: np.where(np.arange(32) < 16, sc, sc * 1e-13),
+    "below 2^-60": lambda sc, rng: np.where(np.arange(32) < 16, sc, sc * 1e-22),
+    "huge": lambda sc, rng: np.where(np.arange(32) < 16, sc, sc * 1e13),
+    "1 in 100 is 100 times the rest": lambda sc, rng: np.where((np.arange(32) >= 16) & (rng.random(sc.shape) < 0.01), sc * 100, sc),
+    "1 in 100 is 1000 times the rest": lambda sc, rng: np.where((np.arange(32) >= 16) & (rng.random(sc.shape) < 0.01), sc * 1000, sc),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(12, 3, 128), (4, 1, 64), (32, 1, 64)])
+@pytest.mark.parametrize("spread", SPREADS)
+@pytest.mark.parametrize("peak", [1.0, 3.0])
+def test_attn_spread_of_scales(native, heads, spread, peak):
+    rng = np.random.default_rng(51)
+    rows = [1, 9, 3]
+    b = kv.Batch(native, rng, heads, [2500, 700, 90], rows, kv.random_tree(rng, rows))
+
+    def change(sc, kc, vc):
+        sc[:] = SPREADS[spread](sc, rng)
+
+    q = (rng.standard_normal((b.n, b.nh, b.hd)) * peak).astype(np.float32)
+    _check_scales(b, rng, change, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("factor", [1e3, 1e6, 1e9, 1e30])
+def test_attn_large_scales_that_a_row_does_not_see(native, hd, factor):
+    """Values of a sibling, of padding and of what lies behind the rows count nowhere, however large."""
+    rng = np.random.default_rng(52)
+    parent = [-1, 0, 0, -2, 1, 2, 0, 4]
+    b = kv.Batch(native, rng, (8, 2, hd), [150], [8], parent)
+    big = [150 + 2, 150 + 3, 150 + 9]  # row 2 (seen by rows 2 and 5), the padding row, behind the rows
+
+    def change(sc, kc, vc):
+        for slot in big:
+            sc[b.table[0, slot // PAGE], :, 16 + slot % PAGE] *= factor
+
+    _check_scales(b, rng, change)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("factor", [1e2, 1e4, 1e8])
+def test_attn_large_scales_that_hardly_count(native, hd, factor):
+    """A slot that is seen with next to no probability and a large V scale takes no accuracy from the others."""
+    rng = np.random.default_rng(53)
+    b = kv.Batch(native, rng, (4, 1, hd), [1200, 40], [1, 2])
+    q = np.abs(rng.standard_normal((b.n, 4, hd))).astype(np.float32) + np.float32(0.5)
+
+    def change(sc, kc, vc):
+        for s, slot in ((0, 300), (0, 1100), (1, 7)):
+            page, w = b.table[s, slot // PAGE], slot % PAGE
+            kc[page, 0, w] = -np.abs(kc[page, 0, w])
+            sc[page, 0, w] *= 4
+            sc[page, 0, 16 + w] *= factor
+
+    _check_scales(b, rng, change, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attn_zero_value_rows(native, hd):
+    """A zero V row (scale 0) takes its probability and adds nothing, the row's only slot or its greatest too."""
+    rng = np.random.default_rng(54)
+    b = kv.Batch(native, rng, (8, 2, hd), [600, 0, 130], [2, 1, 3])
+    zero = [(0, slot) for slot in range(0, 600, 3)] + [(1, 0), (2, 5), (2, 130)]
+    q = rng.standard_normal((b.n, 8, hd)).astype(np.float32)
+
+    def change(sc, kc, vc):
+        for s, slot in zero:
+            page, w = b.table[s, slot // PAGE], slot % PAGE
+            sc[page, :, 16 + w] = 0.0
+            vc[page, :, w] = 0
+        page = b.table[2, 0]  # slot 5 of sequence 2: the greatest score of head 0's rows
+        kc[page, 0, 5] = np.clip(np.round(q[3:, :4].mean((0, 1)) * 200), -127, 127)
+
+    _check_scales(b, rng, change, q)
+
+
+@pytest.mark.gpu
+def test_attn_scales_that_no_append_writes(native):
+    """A row that sees an infinite or NaN scale, or a V scale below zero, gets NaN; the others do not."""
+    rng = np.random.default_rng(56)
+    b = kv.Batch(native, rng, (4, 1, 64), [140], [6], [-1, 0, 0, 0, 0, 0])
+    values = [(0, np.inf), (16, np.inf), (16, -1.0), (0, np.nan)]
+
+    def change(sc, kc, vc):
+        for j, (at, x) in enumerate(values):
+            slot = 141 + j
+            sc[b.table[0, slot // PAGE], :, at + slot % PAGE] = x
+
+    _scaled_pool(b, rng, change)
+    out = b.attn(rng.standard_normal((6, 4, 64)).astype(np.float32)).cpu().numpy().reshape(6, -1)
+    nan = np.isnan(out)
+    assert nan[1:5].all() and not nan[[0, 5]].any()

@@ -25,25 +25,18 @@ __device__ __forceinline__ float kv8_scale(double amax, double* inv) {
   return sc;
 }
 
-// Greatest of the lanes' non-negative doubles: their bit patterns are ordered.
-__device__ __forceinline__ double warp_max_abs(double v) {
-  const uint32_t hi = (uint32_t)__double2hiint(v), lo = (uint32_t)__double2loint(v);
-  const uint32_t mh = __reduce_max_sync(0xffffffffu, hi);
-  const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? lo : 0u);
-  return __hiloint2double((int)mh, (int)ml);
-}
-// The greatest magnitude of a row (an infinity if it holds a NaN or one).
+// The greatest magnitude of a row (an infinity or a NaN if it holds one): bit patterns of magnitudes are
+// ordered, the upper words meet first.
 template <int E>
 __device__ __forceinline__ double row_max(const double (&y)[E]) {
-  double a = 0.0;
-  bool fin = true;
+  uint32_t hi = 0, lo = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const double m = fabs(y[e]);
-    fin = fin && m <= 1.7976931348623157e308;
-    a = m > a ? m : a;
-  }
-  return warp_max_abs(fin ? a : __hiloint2double(0x7ff00000, 0));
+  for (int e = 0; e < E; e++) hi = max(hi, (uint32_t)__double2hiint(y[e]) & 0x7fffffffu);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    if (((uint32_t)__double2hiint(y[e]) & 0x7fffffffu) == hi) lo = max(lo, (uint32_t)__double2loint(y[e]));
+  return __hiloint2double((int)hi, (int)__reduce_max_sync(0xffffffffu, lo));
 }
 template <int E>
 __device__ __forceinline__ double row_max(const float (&x)[E]) {  // NaN patterns lie above the infinities
@@ -102,16 +95,45 @@ __device__ __forceinline__ void kv8_put(const T (&y)[KV8_HEADS][HD / 32], int co
   if (lane < count) *reinterpret_cast<float*>(blk + lane * kv8_block_bytes(HD) + (V ? kv8_vs_off(HD, w) : kv8_ks_off(HD, w))) = sc;
   // only the rounding of a subnormal scale is coarse enough to leave a quotient above 127
   const bool tiny = __any_sync(0xffffffffu, sc < 1.17549435e-38f && sc > 0.0f);
+  const bool odd = tiny || __any_sync(0xffffffffu, !(sc >= 0.0f));  // or a NaN among them
   const int i0 = HeadRow<HD>::dim(0);
   uint8_t* bk = blk + (V ? kv8_v_off(HD, w, i0) : kv8_k_off(HD, w, i0));
 #pragma unroll
   for (int g = 0; g < KV8_HEADS; g++) {
     if (g >= count) break;
-    const double s = __shfl_sync(0xffffffffu, inv, g);
-    uint8_t* b = bk + g * kv8_block_bytes(HD);
+    uint8_t* to = bk + g * kv8_block_bytes(HD);
     int q[E];
+    // y / scale, correctly rounded: the product with the rounded inverse is an ulp off at times, which moves
+    // what lies half-way between two codes (Markstein's correction, "Computation of elementary functions on
+    // the IBM RISC System/6000 processor", 1990). inv = 0: codes 0.
+    auto quotients = [&]() {
+      const double s = __shfl_sync(0xffffffffu, inv, g), sg = (double)__shfl_sync(0xffffffffu, sc, g), by = s > 0.0 ? sg : 0.0;
 #pragma unroll
-    for (int e = 0; e < E; e++) q[e] = kv8_round(__dmul_rn((double)y[g][e], s));
+      for (int e = 0; e < E; e++) {
+        const double v = (double)y[g][e], t = __dmul_rn(v, s);
+        q[e] = kv8_round(fma(fma(-t, by, v), s, t));
+      }
+    };
+    if constexpr (V) {
+      // In f32 the quotient is off by 2 * 2^-24 * 127 < 1e-4 at most: the code is sure where it lies further
+      // than that from half-way between two, which leaves one head's row in 40.
+      const float s1 = __shfl_sync(0xffffffffu, (float)inv, g);
+      const f32x2 s2 = pack2(s1, s1), up2 = pack2(12582912.0f, 12582912.0f), down2 = pack2(-12582912.0f, -12582912.0f);
+      float off = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        // + 1.5 * 2^23: the integer in the low bits
+        const f32x2 t = mul2(pack2((float)y[g][e], (float)y[g][e + 1]), s2), r = add2(t, up2);
+        float a, b;
+        unpack2(r, a, b);
+        q[e] = __float_as_int(a), q[e + 1] = __float_as_int(b);
+        unpack2(fma2(add2(r, down2), pack2(-1.0f, -1.0f), t), a, b);
+        off = fmaxf(off, fmaxf(fabsf(a), fabsf(b)));
+      }
+      if (odd || __any_sync(0xffffffffu, off > 0.4999f)) quotients();
+    } else {
+      quotients();
+    }
     if (tiny) {
 #pragma unroll
       for (int e = 0; e < E; e++) q[e] = min(max(q[e], -127), 127);
@@ -121,11 +143,11 @@ __device__ __forceinline__ void kv8_put(const T (&y)[KV8_HEADS][HD / 32], int co
       const int di = (e / H) * (HD / 2) + e % H;  // from the lane's first dim
       if constexpr (V) {
         if (stage) stage[(g * HD + i0 + di) * KV8_PITCH + w] = (uint8_t)q[e];
-        else b[di * KV8_PAGE] = (uint8_t)q[e];
+        else to[di * KV8_PAGE] = (uint8_t)q[e];
       } else if constexpr (H == 1) {
-        b[di * 8] = (uint8_t)q[e];  // 16 dims on are 128 bytes on
+        to[di * 8] = (uint8_t)q[e];  // 16 dims on are 128 bytes on
       } else if (e % 2 == 0) {
-        *reinterpret_cast<uint16_t*>(b + (e / H) * (HD / 2) * 8) = (uint16_t)((q[e] & 255) | (q[e + 1] & 255) << 8);
+        *reinterpret_cast<uint16_t*>(to + (e / H) * (HD / 2) * 8) = (uint16_t)((q[e] & 255) | (q[e + 1] & 255) << 8);
       }
     }
   }
@@ -136,8 +158,8 @@ __device__ __forceinline__ void kv8_put(const T (&y)[KV8_HEADS][HD / 32], int co
 // g). k runs in f64: a code sits at a rounding border of its row's scale, and f32 sums in another order
 // would move codes by one. The next task's rows come by asynchronous copies meanwhile. The V codes of a
 // full page are turned round in shared memory, so that they leave as 16-byte columns; a page that the call
-// fills in part gets its bytes one by one. 21,000 rows of 16 q and 8 kv heads of 128 dims take 108 us, 560
-// MB, 0.80 of measured HBM: issue slots are 72% busy, most of it with the f64 work on k and the codes.
+// fills in part gets its bytes one by one. 21,000 rows of 16 q and 8 kv heads of 128 dims take 110 us, 560
+// MB, 0.78 of measured HBM: issue slots are 72% busy, most of it with the f64 work on k and the codes.
 template <int HD>
 __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_constant__ hg_kv8_cache C,
                                                               const __grid_constant__ hg_rows R,

@@ -268,3 +268,41 @@ def test_attn_scales_that_no_append_writes(native):
     out = b.attn(rng.standard_normal((6, 4, 64)).astype(np.float32)).cpu().numpy().reshape(6, -1)
     nan = np.isnan(out)
     assert nan[1:5].all() and not nan[[0, 5]].any()
+
+
+# ---------------------------------------------------------------------------------------------
+# codes at a rounding border
+# ---------------------------------------------------------------------------------------------
+def tie_rows(hd):
+    """V rows whose values lie half-way between two codes of their scale: (k + 1/2) scale and the greatest,
+    127 scale, with scales for which x * (1 / scale) in f64 is off the border on either side."""
+    rows = []
+    for scale in (49.0, 98.0 * 2.0 ** -9, 103.0, 107.0, 161.0 * 2.0 ** 4, 187.0, 65521.0, 1.0, 0.75):
+        x = (np.arange(hd) % 127 + 0.5) * scale * np.where(np.arange(hd) % 3, 1, -1)
+        x[hd // 2] = 127 * scale
+        assert (x == x.astype(np.float32)).all()
+        rows.append(x)
+    return np.array(rows, np.float32)
+
+
+def test_tie_rows_tell_a_product_from_a_quotient():
+    x = tie_rows(128).astype(np.float64)
+    scale = np.abs(x).max(-1, keepdims=True) / 127
+    assert (np.round(x * (1 / scale)) != np.round(x / scale)).sum() > 50
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_codes_half_way_between_two_go_to_the_even_one(native, hd):
+    x = tie_rows(hd)
+    rng = np.random.default_rng(57)
+    b = kv.Batch(native, rng, (1, 1, hd), [3], [len(x)])
+    qkv = rng.standard_normal((len(x), 3, hd)).astype(np.float32)
+    qkv[:, 2] = x
+    one = np.ones(hd, np.float32)
+    b.append(qkv, (one, one), kv.rope_tables(hd, 32))
+    _, vc, sc = kv.unpack(b.pool_np(), hd)
+    slot = 3 + np.arange(len(x))
+    page, w = b.table[0, slot // PAGE], slot % PAGE
+    code, scale = kv.quantised(x)
+    assert np.array_equal(sc[page, 0, 1, w], scale) and np.array_equal(vc[page, 0, w], code)

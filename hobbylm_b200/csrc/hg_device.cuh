@@ -175,9 +175,9 @@ __device__ __forceinline__ float key2f(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 // argmax key: high word = value key, low word = ~index so that the lowest index wins ties
-// (sample.rs:53-64 keeps the first maximum).
+// (sample.rs:53-64 keeps the first maximum; -0 and +0 are equal).
 __device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t idx) {
-  return ((unsigned long long)f2key(v) << 32) | (unsigned long long)(0xffffffffu - idx);
+  return ((unsigned long long)f2key(v == 0.0f ? 0.0f : v) << 32) | (unsigned long long)(0xffffffffu - idx);
 }
 
 }  // namespace hg

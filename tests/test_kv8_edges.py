@@ -306,3 +306,28 @@ def test_codes_half_way_between_two_go_to_the_even_one(native, hd):
     page, w = b.table[0, slot // PAGE], slot % PAGE
     code, scale = kv.quantised(x)
     assert np.array_equal(sc[page, 0, 1, w], scale) and np.array_equal(vc[page, 0, w], code)
+
+
+# ---------------------------------------------------------------------------------------------
+# logit rules: zeros of both signs
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [40, 5003, 50304])
+def test_rules_minus_zero_equals_zero(native, vocab):
+    """The first of the greatest wins where -0.0 and +0.0 are the greatest: in different threads and CTAs,
+    in the stream or listed, a zero that a penalty made among them."""
+    rng = np.random.default_rng(58)
+    pairs = [(0, vocab - 1), (3, 4), (5, 6 + vocab // 2), (vocab // 2, vocab // 2 + 9)]
+    for first, second in pairs:
+        for listed in ([], [first], [second], [first, second]):
+            x = -1 - np.abs(rng.standard_normal((3, vocab))).astype(np.float32)
+            x[0, first], x[0, second] = -0.0, 0.0
+            x[1, first], x[1, second] = 0.0, -0.0
+            x[2, first], x[2, second] = -1e-45, 0.0  # listed: halved to -0.0
+            hists = [listed] * 3
+            rep = np.full(3, 0.5, np.float32)
+            out, nxt = kv._rules(native, x, [1] * 3, hists=hists, rep=rep)
+            zero = np.zeros(3, np.float32)
+            want, ids, _ = kv.rules_ref(x, kv.offsets([1] * 3), None, None, hists, rep, zero, zero, [[]] * 3, vocab, [None] * 3, exact=False)
+            assert np.array_equal(out, want) and np.array_equal(nxt, ids), (first, second, listed)
+            assert nxt.tolist()[:2] == [first, first]

@@ -209,28 +209,25 @@ __global__ void __launch_bounds__(32 * KV8_WARPS, 3) k_kv8_append(const __grid_c
   place(next);
   fetch(next, mine);
   uint8_t* page = kv8_block(C, s, base, 0);
-  if (threadIdx.x < nr) {
-    const int j = j0 + threadIdx.x;
-    long long pos = (long long)sp.start + j;
-    if (R.parent) {
-      int up = kv8_parent(R, sp, j);
-      if (up == -2) {
-        pos = -1;
-      } else {
-        pos = sp.start;
-        while (up >= 0) {  // strictly down: at most j steps; a padding ancestor ends the path
-          const int q = kv8_parent(R, sp, up);
-          if (q == -2) break;
-          pos++;
-          up = q;
-        }
-      }
-    }
+  auto put_pos = [&](int r, long long pos) {
     if (pos >= 0 && (pos >= A.max_pos || !page)) {
       kv8_flag(R.err, HG_ERR_CONTEXT);
       pos = -1;
     }
-    pos_s[threadIdx.x] = (int)pos;
+    pos_s[r] = (int)pos;
+  };
+  if (!R.parent) {
+    if (threadIdx.x < nr) put_pos(threadIdx.x, (long long)sp.start + j0 + threadIdx.x);
+  } else {
+    for (int r = threadIdx.x >> 4; r < nr; r += blockDim.x >> 4) {  // half a warp a row
+      int depth = -1;  // a padding ancestor ends the path
+      for (int at = j0 + r; at >= 0;) {
+        const PathRun run = kv8_run<16>(R, sp, at);
+        depth += run.len;
+        at = run.next;
+      }
+      if ((lane & 15) == 0) put_pos(r, depth < 0 ? -1 : (long long)sp.start + depth);
+    }
   }
   __syncthreads();
   uint8_t* v_stage = reinterpret_cast<uint8_t*>(rows_s + warps * 2 * KV8_HEADS * HD);

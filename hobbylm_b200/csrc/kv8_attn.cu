@@ -101,6 +101,7 @@ struct KaSmall {
   int lim[R];                // row r sees the slots below, and the tree slots of `vis`; -1: padding
   int node[R], off[R];       // row r's node within its block, its q head's place behind the block's first
   uint32_t vis[R][4];        // slots of the current tile that row r's path holds
+  int at[R];                 // where a node's path goes on below the tiles looked at
   uint32_t pages[4];         // per stage: which of the tile's pages are there
   uint32_t tmem;
   int fail;
@@ -377,13 +378,13 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
       const int last = ka_last(u);
       auto page_of = [&](int tile) -> const uint8_t* {
         const long long slot = (long long)tile * KA_TILE + lane * KV8_PAGE;
-        if (lane >= KA_PAGES || tile >= last || slot >= u.seen) return nullptr;
+        if (lane >= KA_PAGES || tile < u.lo || slot >= u.seen) return nullptr;
         const uint8_t* b = kv8_block(A.C, u.s, slot, u.kvh);
         if (!b) kv8_flag(A.R.err, HG_ERR_CONTEXT);
         return b;
       };
-      const uint8_t* src = page_of(u.lo);
-      for (int tile = u.lo; tile < last; tile++, n++) {
+      const uint8_t* src = page_of(last - 1);
+      for (int tile = last - 1; tile >= u.lo; tile--, n++) {
         const int k = n % STAGES;
         const uint32_t past = (n / STAGES - 1) & 1;
         if (n >= STAGES) ka_wait(&sm.empty_k[k], past, &sm.fail);
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             mbar_arrive(&sm.full_k[k]);
           }
         }
-        const uint8_t* next = page_of(tile + 1);
+        const uint8_t* next = page_of(tile - 1);
         if (n >= STAGES) ka_wait(&sm.empty_v[k], past, &sm.fail);
         if (lane < KA_PAGES) {
           if (src) {
@@ -474,6 +475,8 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           lim = kv8_parent(A.R, u.sp, j) == -2 ? -1 : (int)min(up_to, (long long)ka_cap(A.C));
         }
         sm.lim[tid] = lim;
+        sm.at[tid] = u.j0 + tid;
+        *reinterpret_cast<uint4*>(sm.vis[tid]) = make_uint4(0, 0, 0, 0);
         sm.m[0][tid] = sm.m[1][tid] = KA_NONE;
       }
 #pragma unroll
@@ -536,7 +539,8 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         tc_fence_after();
         issue_scores(n % STAGES);
       }
-      for (int tile = u.lo; tile < last; tile++, n++) {
+      // from the last tile down, so that a path is walked once and not from its row again for every tile
+      for (int tile = last - 1; tile >= u.lo; tile--, n++) {
         const int k = n % STAGES;
         const int slot = tile * KA_TILE + ti;
         ka_wait(&sm.full_k[k], (n / STAGES) & 1, &sm.fail);  // the scales (the codes are the MMAs')
@@ -554,26 +558,22 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
         const bool whole = there == (1u << KA_PAGES) - 1 && (tile + 1) * KA_TILE <= u.sp.start;
         const bool tree = A.R.parent && (tile + 1) * KA_TILE > u.sp.start;
         if (tree) {
-          // the path of each node, as bits of this tile
-          if (tid < R) {
-            uint32_t v[4] = {0, 0, 0, 0};
-            const int node = sm.node[tid];
-            if (node < u.nodes) {
-              for (int at = u.j0 + node; at >= 0;) {
-                const int up = kv8_parent(A.R, u.sp, at);
-                if (up == -2) break;
-                const long long b = (long long)u.sp.start + at - (long long)tile * KA_TILE;
-                if (b < 0) break;  // ancestors lie below
-                if (b < KA_TILE) {
-#pragma unroll
-                  for (int i = 0; i < 4; i++)
-                    if ((b >> 5) == i) v[i] |= 1u << (b & 31);
-                }
-                at = up;
-              }
+          // the path of each node, as bits of this tile: half a warp a node, lanes 0..3 a word each
+          for (int node = tid >> 4; node < u.nodes; node += S::COMPUTE / 16) {
+            const int word = lane & 15;
+            uint32_t v = 0;
+            int at = sm.at[node];
+            while (at >= 0) {
+              const long long b = (long long)u.sp.start + at - (long long)tile * KA_TILE;  // bit of row `at`
+              if (b < 0) break;  // the path goes on in a tile below
+              const PathRun run = kv8_run<16>(A.R, u.sp, at);
+              const int hi = (int)min(b - 32 * word, 31ll), lo = (int)max(b - run.len + 1 - 32 * word, 0ll);
+              if (word < 4 && lo <= hi) v |= (0xffffffffu >> (31 - (hi - lo))) << lo;
+              at = run.len > b + 1 ? at - (int)b - 1 : run.next;
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) sm.vis[tid][i] = v[i];
+            if (word < 4)
+              for (int r = node * A.g; r < (node + 1) * A.g; r++) sm.vis[r][word] = v;
+            if (word == 0) sm.at[node] = at;
           }
           bar_all();
         }
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
           const float4 v = make_float4(warp_fmax(x[0]), warp_fmax(x[1]), warp_fmax(x[2]), warp_fmax(x[3]));
           if (lane == 0) *reinterpret_cast<float4*>(&sm.wmax[quad][rb + r]) = v;
         }
-        if (tile > u.lo) add_out(n - 1);  // the previous tile's sums, while the others get here
+        if (tile < last - 1) add_out(n - 1);  // the previous tile's sums, while the others get here
         bar_group();
         const int now = n & 1;
         if (__any_sync(0xffffffffu, !fine)) {
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(KaShape<HD, R>::THREADS, KaShape<HD, R>::PER_S
             tc_mma_acc(tm + S::COL_O, tc_desc(a + i * 32 * HD, 16 * HD, 128, 0),
                        tc_desc(bp_a + i * 2 * S::PITCH, S::PITCH, 128, 0), IDESC_O, i > 0);
           tc_commit(&sm.obar);
-          if (tile + 1 < last) {  // the next tile's scores meanwhile
+          if (tile > u.lo) {  // the next tile's scores meanwhile
             ka_wait(&sm.full_k[(n + 1) % STAGES], ((n + 1) / STAGES) & 1, &sm.fail);
             issue_scores((n + 1) % STAGES);
           }

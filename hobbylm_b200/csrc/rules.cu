@@ -187,19 +187,15 @@ __device__ __forceinline__ unsigned long long rules_run(const hg_rows& R, const 
     }
     for (int at = A.j; at >= 0;) {  // the same for every thread
       __syncthreads();
-      if (tid == 0) {
+      if (warp == 0) {
         int n = 0, up = at;
-        while (up >= 0 && n < LR_PATH) {
-          const int next = kv8_parent(R, A.sp, up);
-          if (next == -2) {
-            up = -1;
-            break;
-          }
-          sh.path[n++] = A.token[up];
-          up = next;
+        while (up >= 0 && n + 32 <= LR_PATH) {
+          const PathRun run = kv8_run<32>(R, A.sp, up);
+          if (lane < run.len) sh.path[n + lane] = A.token[up - lane];
+          n += run.len;
+          up = run.next;
         }
-        sh.path_n = n;
-        sh.path_at = up;
+        if (lane == 0) sh.path_n = n, sh.path_at = up;
       }
       __syncthreads();
       at = sh.path_at;

@@ -331,3 +331,91 @@ def test_rules_minus_zero_equals_zero(native, vocab):
             want, ids, _ = kv.rules_ref(x, kv.offsets([1] * 3), None, None, hists, rep, zero, zero, [[]] * 3, vocab, [None] * 3, exact=False)
             assert np.array_equal(out, want) and np.array_equal(nxt, ids), (first, second, listed)
             assert nxt.tolist()[:2] == [first, first]
+
+
+# ---------------------------------------------------------------------------------------------
+# long paths given by parents
+# ---------------------------------------------------------------------------------------------
+def deep_tree(rng, n, kind):
+    if kind == "chain":
+        return [j - 1 for j in range(n)]
+    if kind == "two chains":  # every other row
+        return [j - 2 if j > 1 else -1 for j in range(n)]
+    if kind == "chain and trees":  # a prompt, drafts behind it
+        return [j - 1 for j in range(n - 40)] + [int(rng.integers(n - 41, n - 40 + j)) for j in range(40)]
+    p = []  # runs with jumps, padding rows, roots
+    for j in range(n):
+        x = rng.random()
+        p.append(j - 1 if x < 0.95 else -2 if x < 0.96 else int(rng.integers(max(-1, j - 70), j)) if j else -1)
+    return p
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(12, 3, 128), (4, 4, 64), (32, 1, 64)])
+@pytest.mark.parametrize("kind", ["chain", "two chains", "chain and trees", "runs"])
+def test_long_paths(native, heads, kind):
+    """Appended and attended: positions by the number of ancestors, visibility by the path, over many tiles."""
+    nh, nkv, hd = heads
+    rng = np.random.default_rng(61)
+    starts, rows = [77, 0, 300], [333, 150, 1]
+    parent = sum((deep_tree(rng, n, kind) if n > 100 else [-1] for n in rows), [])
+    b = kv.Batch(native, rng, heads, starts, rows, parent)
+    qkv = rng.standard_normal((b.n, nh + 2 * nkv, hd)).astype(np.float32)
+    one, rope = np.ones(hd, np.float32), kv.rope_tables(hd, 512)
+    q = b.append(qkv, (one, one), rope).cpu().numpy().reshape(-1, nh, hd)
+    depth = np.array([len(kv.path_of(b.parent, b.row_off[s], j)) - 1 for s in range(3) for j in range(rows[s])])
+    live = depth >= 0
+    pos = (b.starts[np.repeat(np.arange(3), rows)] + depth)[live]
+    want, amp = kv.norm_rope(qkv[live, :nh], one, 1e-5, rope[0][pos][:, None], rope[1][pos][:, None])
+    assert (np.abs(q[live] - want) <= 24 * U * amp + 1e-30).all() and (q[~live] == 0).all()
+    kv._check_attn(b, rng)
+
+
+@pytest.mark.gpu
+def test_a_chain_of_parents_is_the_chain(native):
+    """The same bits as parent = NULL, and in the same order of time."""
+    import torch
+
+    rng = np.random.default_rng(62)
+    heads, n = (8, 2, 64), 2500
+    q = kv.dev(rng.standard_normal((n, 8, 64)).astype(np.float32))
+    qkv = rng.standard_normal((n, 12, 64)).astype(np.float32)
+    one, rope = np.ones(64, np.float32), kv.rope_tables(64, 2600)
+    got, ms = [], []
+    for parent in (None, [j - 1 for j in range(n)]):
+        b = kv.Batch(native, np.random.default_rng(63), heads, [50], [n], parent)
+        b.fill(np.random.default_rng(64))
+        qs = b.append(qkv, (one, one), rope)
+        out = b.attn(q).clone()
+        scratch, best = b.scratch, 1e9
+        for _ in range(3):
+            a, e = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            b.attn(q, None, scratch, out)
+            e.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(e))
+        got.append((qs, b.pool.clone(), out.clone()))
+        ms.append(best)
+        assert b.err_code() == 0
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    print(f"chain {ms[0]:.3f} ms, by parents {ms[1]:.3f} ms")
+    # a row block walks each row's path once, at most 2500 rows, 16 a step, beside its 20 tiles: as many
+    # steps of a load each as its tiles take times eight; a walk per tile took 46 times the chain's time
+    assert ms[1] <= 8 * ms[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["chain", "two chains", "runs"])
+def test_rules_long_paths(native, kind):
+    rng = np.random.default_rng(65)
+    n, v = 700, 300
+    parent = deep_tree(rng, n, kind)
+    logits = rng.standard_normal((n, v)).astype(np.float32)
+    token = rng.integers(0, v, n).tolist()
+    rep, freq, zero = np.array([1.1], np.float32), np.array([0.25], np.float32), np.zeros(1, np.float32)
+    out, nxt = kv._rules(native, logits, [n], parent, token, [[3]], rep, freq)
+    want, ids, _ = kv.rules_ref(logits, kv.offsets([n]), np.array(parent), token, [[3]], rep, freq, zero, [[]], v, [None] * n, exact=False)
+    live = np.array(parent) != -2
+    assert np.array_equal(out[live], want[live]) and np.array_equal(nxt, ids)

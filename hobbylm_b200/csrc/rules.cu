@@ -351,8 +351,9 @@ __global__ void __launch_bounds__(LR_THREADS, 4) k_logits_rules(const __grid_con
   if (s < 0) return;  // behind the last sequence (the whole cluster leaves)
   RulesRow w;
   const int h0 = A.hist_off ? A.hist_off[s] : 0, b0 = A.bias_off ? A.bias_off[s] : 0;
-  w.hn = A.hist_off ? A.hist_off[s + 1] - h0 : 0;
-  w.bn = A.bias_off ? A.bias_off[s + 1] - b0 : 0;
+  // below 0 (no entries) where the offsets descend or are below 0 themselves
+  w.hn = A.hist_off ? (int)((uint32_t)A.hist_off[s + 1] - (uint32_t)h0) | h0 >> 31 : 0;
+  w.bn = A.bias_off ? (int)((uint32_t)A.bias_off[s + 1] - (uint32_t)b0) | b0 >> 31 : 0;
   w.rep = A.rep_penalty ? A.rep_penalty[s] : 1.0f;
   w.freq = A.freq_penalty ? A.freq_penalty[s] : 0.0f;
   w.pres = A.pres_penalty ? A.pres_penalty[s] : 0.0f;
@@ -374,8 +375,9 @@ __global__ void __launch_bounds__(LR_THREADS, 4) k_logits_rules(const __grid_con
   w.token = A.token ? A.token + w.sp.r0 : nullptr;
   w.valid = A.valid > 0 ? min(A.valid, A.vocab) : A.vocab;
   const int lo = part * per, hi = min(A.vocab, lo + per);
-  unsigned long long best = (long long)w.hn + w.j + 1 < LR_LONG ? rules_run<VEC, false>(R, w, sh, words_s, room, lo, hi)
+  unsigned long long best = (long long)max(w.hn, 0) + w.j + 1 < LR_LONG ? rules_run<VEC, false>(R, w, sh, words_s, room, lo, hi)
                                                                : rules_run<VEC, true>(R, w, sh, words_s, room, lo, hi);
+  if (tid == 0 && (w.hn | w.bn) < 0) kv8_flag(R.err, HG_ERR_INVALID);
   if (!A.next_ids) return;
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) sh.red[warp] = best;

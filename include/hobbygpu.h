@@ -329,8 +329,8 @@ int hg_op_kv_attn(const hg_kv_attn_args* a, void* scratch, void* stream);
  *
  * Pointers in these structs are device memory, 4-byte aligned (float rows read or written whole 16-byte
  * aligned); the call runs on the device that holds the pool (for the rules: the logits). Arrays in
- * device memory are checked on the device: what breaks a rule is left out as described, and *err, when
- * given, is set to an HG_ERR_* code and never cleared. Calls neither allocate nor synchronise, and can
+ * device memory are checked on the device as far as their sizes are known: what breaks a rule is left out as
+ * described, and *err, when given, is set to an HG_ERR_* code and never cleared. Calls neither allocate nor synchronise, and can
  * be captured into a CUDA graph. */
 
 /* The cache of one layer. Pages hold 16 slots; the block of kv head h in page p starts at
@@ -416,12 +416,13 @@ typedef struct {
   int64_t ld, ld_out;            /* floats between rows (0: vocab) */
   int32_t* next_ids;             /* [n_rows] or NULL */
   const int32_t* token;          /* [n_rows] the drafted token of each row, or NULL (none counted) */
-  const int32_t* hist_off;       /* [n_seqs + 1] or NULL */
+  const int32_t* hist_off;       /* [n_seqs + 1] or NULL; offsets that descend or are below 0: no entries for
+                                  * that sequence (err HG_ERR_INVALID); hist must reach to the last one */
   const int32_t* hist;           /* ids */
   const float* rep_penalty;      /* [n_seqs] each, or NULL */
   const float* freq_penalty;
   const float* pres_penalty;
-  const int32_t* bias_off;       /* [n_seqs + 1] or NULL */
+  const int32_t* bias_off;       /* as hist_off */
   const int32_t* bias_id;
   const float* bias;
   const uint32_t* mask;          /* rows of mask_words words, bit i % 32 of word i / 32 = id i is allowed; or NULL */

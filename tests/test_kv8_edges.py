@@ -419,3 +419,34 @@ def test_rules_long_paths(native, kind):
     want, ids, _ = kv.rules_ref(logits, kv.offsets([n]), np.array(parent), token, [[3]], rep, freq, zero, [[]], v, [None] * n, exact=False)
     live = np.array(parent) != -2
     assert np.array_equal(out[live], want[live]) and np.array_equal(nxt, ids)
+
+
+@pytest.mark.gpu
+def test_rules_list_offsets_out_of_order(native):
+    """Offsets below zero and descending ones: no entries for that sequence, reported; the others as ever."""
+    import torch
+
+    rng = np.random.default_rng(59)
+    v, n = 500, 4
+    x = rng.standard_normal((n, v)).astype(np.float32)
+    hist, bias_id = rng.integers(0, v, 30), rng.integers(0, v, 30)
+    t = {k: kv.dev(a) for k, a in (("logits", x), ("hist", hist.astype(np.int32)), ("bias_id", bias_id.astype(np.int32)),
+                                   ("bias", np.ones(30, np.float32)), ("rep_penalty", np.full(n, 1.5, np.float32)))}
+    row_off, err = kv.dev(kv.offsets([1] * n)), torch.zeros(1, dtype=torch.int32, device="cuda")
+    r = native.Rows(n_seqs=n, n_rows=n, max_rows=1, row_off=kv.ptr(row_off), err=kv.ptr(err))
+    good, cases = [0, 10, 10, 20, 30], ([0, 10, 10, 20, 30], [-5, 10, 10, 20, 30], [0, 10, 20, 15, 30], [-9, -4, 10, 20, 30])
+    for which in ("hist_off", "bias_off"):
+        for off in cases:
+            used = {k: kv.dev(np.array(off if k == which else good, np.int32)) for k in ("hist_off", "bias_off")}
+            out = torch.zeros((n, v), device="cuda")
+            err.zero_()
+            a = native.LogitsRules(vocab=v, out=kv.ptr(out), **{k: kv.ptr(b) for k, b in {**t, **used}.items()})
+            native.check(native.lib().hg_op_logits_rules(C.byref(r), C.byref(a), None))
+            lists = [[slice(o[s], o[s + 1]) if 0 <= o[s] <= o[s + 1] else slice(0, 0) for s in range(n)]
+                     for o in ((off, good) if which == "hist_off" else (good, off))]
+            hists = [hist[c].tolist() for c in lists[0]]
+            biases = [[(int(i), 1.0) for i in bias_id[c]] for c in lists[1]]
+            zero = np.zeros(n, np.float32)
+            want, _, _ = kv.rules_ref(x, kv.offsets([1] * n), None, None, hists, np.full(n, 1.5, np.float32), zero, zero, biases, v, [None] * n, exact=False)
+            assert np.array_equal(out.cpu().numpy(), want)
+            assert int(err.cpu()[0]) == (0 if off == good else INVALID)

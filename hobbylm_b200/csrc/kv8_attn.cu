@@ -40,12 +40,13 @@
 // is bounded; when one gives up, the CTA reports HG_ERR_TIMEOUT, its other waits give up soon too, and it
 // waits (bounded) for its copies and last MMAs before it frees its tensor memory and returns.
 //
-// Measured: 256 sequences of 1024 to 8192 slots (12 q heads, 3 kv heads, 128 dims) 147-152 us, 5.9 TB/s
+// Measured: 256 sequences of 1024 to 8192 slots (12 q heads, 3 kv heads, 128 dims) 150 us, 5.9 TB/s
 // of cache, 0.90 of measured HBM (R = 4, three CTAs an SM: bound by HBM). 32 trees of 64 nodes over 900
 // to 7000 slots 264 us, 190 TFLOP/s of f32-like products (R = 32, two CTAs of 288 threads an SM): bound
 // by the instructions between the products, about 50 per (slot, row): put four digits together, scale,
-// maximum, exponential, sum, three digits again, add the value sums. Issue slots are 55% busy at 17 warps
-// an SM, which 96 registers a thread allow; the tensor pipe 13%.
+// maximum, exponential, sum, three digits again, add the value sums. Issue slots are 57% busy at 17 warps
+// an SM, the tensor pipe 16%. The ninth warp leaves the others 96 registers, and some are spilled (52 bytes
+// a thread at R = 32, 8 at 16).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -871,7 +872,8 @@ void check_attn(const hg_kv8_cache* c, const hg_rows* r, int n_heads) {
 // Rows of a block: 4, 8, 16 or 32, whichever makes a ragged batch cheapest. A block's cost, the mean of
 // the call's time per block at 64 and at 256 rows a kv head (32 sequences of 900 to 7000 slots, 12 q
 // heads, 3 kv heads, 128 dims; us): 11.7, 13.8, 23.3 and 36.7. The whole calls took 752, 433, 363 and 267
-// us at 256 rows, 31.1, 28.4, 34.0 and 48.0 us with the one block that the size just fills. The
+// us at 256 rows, 31.1, 28.4, 34.0 and 48.0 us with the one block that the size just fills. (64 dims: by
+// assumption the same.) The
 // sequences' row counts lie between 1 and max_rows; they are taken as spread evenly around their mean.
 int block_rows(const hg_rows* r, int g) {
   const double hi = std::min(r->max_rows, r->n_rows), mean = std::min(hi, (double)r->n_rows / r->n_seqs);

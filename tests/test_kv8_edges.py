@@ -401,8 +401,8 @@ def test_a_chain_of_parents_is_the_chain(native):
     for x, y in zip(*got):
         assert torch.equal(x, y)
     print(f"chain {ms[0]:.3f} ms, by parents {ms[1]:.3f} ms")
-    # a row block walks each row's path once, at most 2500 rows, 16 a step, beside its 20 tiles: as many
-    # steps of a load each as its tiles take times eight; a walk per tile took 46 times the chain's time
+    # a row block walks its rows' paths once, at most 2500 rows at 16 a load (157 loads), beside up to 20 tiles
+    # of a dozen dependent steps each; a walk of every path for every tile took 46 times the chain's time
     assert ms[1] <= 8 * ms[0]
 
 

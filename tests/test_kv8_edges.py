@@ -11,6 +11,7 @@ import pytest
 import test_kv8 as kv
 
 U, PAGE, INVALID, CONTEXT = kv.U, kv.PAGE, kv.INVALID, kv.CONTEXT
+EPS = float(np.float32(1e-5))  # as the calls take it
 
 
 @pytest.mark.gpu
@@ -42,8 +43,8 @@ def test_append_between_padding_rows(native, heads):
     assert 0.3 < live.mean() < 0.6 and (pos >= max_pos).any()
     at, page, w = pos[live], b.table[seq[live], slot[live] // PAGE], slot[live] % PAGE
     cos, sin = rope[0][at][:, None], rope[1][at][:, None]
-    qr, amp = kv.norm_rope(qkv[live, :nh], gains[0], 1e-5, cos, sin)
-    kr, _ = kv.norm_rope(qkv[live, nh:nh + nkv], gains[1], 1e-5, cos, sin)
+    qr, amp = kv.norm_rope(qkv[live, :nh], gains[0], EPS, cos, sin)
+    kr, _ = kv.norm_rope(qkv[live, nh:nh + nkv], gains[1], EPS, cos, sin)
     want = [kv.quantised(kr), kv.quantised(qkv[live, nh + nkv:])]
     a_t = None
     for _ in range(4):
@@ -366,7 +367,7 @@ def test_long_paths(native, heads, kind):
     depth = np.array([len(kv.path_of(b.parent, b.row_off[s], j)) - 1 for s in range(3) for j in range(rows[s])])
     live = depth >= 0
     pos = (b.starts[np.repeat(np.arange(3), rows)] + depth)[live]
-    want, amp = kv.norm_rope(qkv[live, :nh], one, 1e-5, rope[0][pos][:, None], rope[1][pos][:, None])
+    want, amp = kv.norm_rope(qkv[live, :nh], one, EPS, rope[0][pos][:, None], rope[1][pos][:, None])
     assert (np.abs(q[live] - want) <= 24 * U * amp + 1e-30).all() and (q[~live] == 0).all()
     kv._check_attn(b, rng)
 
